@@ -1,0 +1,40 @@
+// The entry of attention for drafted tokens: checks, and which form takes a call.
+#include <algorithm>
+
+#include "tree_attention.cuh"
+
+using namespace srlm;
+
+static tree::Form form_of(int hd, int sms) { return tree::simt_form(hd, sms); }
+
+// float32 words of workspace that srlm_tree_attention wants for these sizes, or -1 where it refuses them.
+extern "C" long long srlm_tree_attention_workspace(int dtype, int nq, int nkv, int hd, int page_size, int max_q_len, int sms) {
+  if ((dtype != DT_F32 && dtype != DT_BF16) || nq <= 0 || nkv <= 0 || nq % nkv || hd <= 0 || hd > 256 || page_size <= 0 ||
+      max_q_len <= 0 || sms <= 0 || (long long)max_q_len * (nq / nkv) > (1 << 24)) {
+    refuse(ST_BAD_SIZE, "tree_attention: dtype=%d nq=%d nkv=%d hd=%d page_size=%d max_q_len=%d (needs nq %% nkv == 0, hd <= 256)",
+           dtype, nq, nkv, hd, page_size, max_q_len);
+    return -1;
+  }
+  const tree::Form f = form_of(hd, sms);
+  return 2ll * f.blocks * f.rows * (hd + 2);
+}
+
+// q, out [T, nq, hd]; caches [num_pages, nkv, page_size, hd]; block_table [n, table_stride]; cu_q [n + 1]; kv_lens [n]; mask
+// [T, words]; positions [T], or null without a window.  max_q_len: no entry has more tokens.  work: as above says.
+extern "C" int srlm_tree_attention(const void* q, const void* k_cache, const void* v_cache, void* out, int dtype, long long num_pages,
+                                   const int* block_table, int table_stride, const int* cu_q, const int* kv_lens, const int* mask,
+                                   int words, const int* positions, int n, int T, int nq, int nkv, int hd, int page_size, float scale,
+                                   int window, int max_q_len, float* work, int sms, int* err_flag, cudaStream_t stream) {
+  if (n <= 0 || T <= 0) return ST_OK;
+  if (srlm_tree_attention_workspace(dtype, nq, nkv, hd, page_size, max_q_len, sms) < 0) return ST_BAD_SIZE;
+  if (words <= 0 || table_stride <= 0 || num_pages <= 0 || num_pages > 0x7fffffff || window < 0 || (window > 0 && !positions) || !work || !err_flag)
+    return refuse(ST_BAD_SIZE, "tree_attention: words=%d table_stride=%d num_pages=%lld window=%d (a window needs the positions)", words,
+                  table_stride, num_pages, window);
+  const tree::Form f = form_of(hd, sms);
+  tree::Args a{q, k_cache, v_cache, out, block_table, table_stride, cu_q, kv_lens, mask, words, std::min(max_q_len, 32 * words), positions, n, T,
+               nq, nkv, hd, page_size, (int)num_pages, scale * 1.4426950408889634f, window, 1, err_flag, work,
+               work + 2ll * f.blocks * f.rows * hd};
+  const int max_rows = max_q_len * (nq / nkv);
+  a.least_tiles = 4;
+  return tree::run_simt(a, dtype, max_rows, sms, stream);
+}

@@ -11,6 +11,7 @@ import ctypes as C
 import functools
 from typing import Optional
 
+import numpy as np
 import torch
 
 from ..errors import ShapeError, Unavailable
@@ -832,6 +833,165 @@ class KernelLibrary:
         else:
             self.paged_attention_rows(q, k_cache, v_cache, out, block_table, ctx.cu_q, ctx.kv_lens, work_list(64),
                                       nq, nkv, hd, page_size, scale, window)
+
+    # ---- drafted tokens, pages of the cache ------------------------------------------------
+    @staticmethod
+    def _here(what, *tensors):
+        """Every tensor (None: not given) lies on the current device: a launch goes to that device's stream."""
+        here = _CURRENT_DEVICE() if _CURRENT_DEVICE is not None else torch.cuda.current_device()
+        for t in tensors:
+            if t is not None and t.get_device() != here:
+                raise ShapeError(f"{what}: a tensor on {t.device}, the current device is cuda:{here}")
+
+    @staticmethod
+    def _ints(what, **tensors):
+        for name, (t, shape) in tensors.items():
+            if t.dtype != torch.int32 or tuple(t.shape) != shape:
+                raise ShapeError(f"{what}: {name} is int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+
+    def draft_tree(self, parents, cu_q, kv_lens, positions, mask, window=0):
+        """What each drafted token of a batch sees of its entry's, from the tokens' parents.
+
+        Entry e's tokens are cu_q[e] .. cu_q[e + 1] - 1; parents int32 [T] holds the place of a token's parent among its
+        entry's tokens, -1 for one without (a parent stands before its children).  Writes positions int32 [T], the entry's
+        committed tokens (kv_lens - its tokens here) plus the token's depth, and mask int32 [T, words]: bit k % 32 of
+        word k / 32 is set iff token k of the entry is the token itself or one it descends from -- under a window, at most
+        window - 1 above it.  words * 32 is at least any entry's number of tokens.  A parent that does not stand before
+        its child counts as none and raises the error word, as do lengths that contradict one another (such an entry is
+        left out)."""
+        T, n = parents.shape[0], kv_lens.shape[0]
+        if mask.dim() != 2 or window < 0:
+            raise ShapeError(f"draft_tree: mask {list(mask.shape)} is [tokens, words], window {window} at least 0")
+        self._ints("draft_tree", parents=(parents, (T,)), cu_q=(cu_q, (n + 1,)), kv_lens=(kv_lens, (n,)),
+                   positions=(positions, (T,)), mask=(mask, (T, mask.shape[1])))
+        args = (_ptr(parents), _ptr(cu_q), _ptr(kv_lens), _ptr(positions), _ptr(mask))
+        self._here("draft_tree", parents, cu_q, kv_lens, positions, mask)
+        self._check(self.lib.srlm_draft_tree(*args, C.c_int(mask.shape[1]), C.c_int(n), C.c_int(T), C.c_int(window),
+                                             _ptr(self._gemm_state(parents.device)[1]), _stream()), "draft_tree")
+
+    def tree_attention(self, q, k_cache, v_cache, out, block_table, cu_q, kv_lens, mask, nq, nkv, hd, page_size, scale,
+                       max_q_len, positions=None, window=0):
+        """Attention of drafted tokens over the paged cache: every token sees its entry's committed keys and, of the
+        entry's own tokens, those that its mask names.
+
+        q, out [T, nq * hd], float32 or bfloat16, of the caches' type; k_cache, v_cache [pages, nkv, page_size, hd]; the
+        tokens' own keys and values stand in the cache already, as the last of each entry's kv_lens.  block_table int32
+        [n, pages of an entry], cu_q int32 [n + 1], kv_lens int32 [n]; mask int32 [T, words] as ``draft_tree`` makes it
+        (any other mask will do: bits of any of the entry's tokens, the token's own among them or not; a token that sees
+        nothing has zeros).  max_q_len: no entry has more tokens.  window > 0: a token sees the committed keys less than
+        window in front of its position (positions int32 [T] is wanted then; the mask carries the window among the
+        tokens).  Rows of q behind cu_q[n] are not read and theirs of out are left as they are.  What stands in places
+        of the cache that a token does not see never reaches its row.  A page number outside the pool, or lengths that
+        contradict one another, raise the error word (such an entry's rows are left, such a page is read as page 0)."""
+        T, n = q.shape[0], kv_lens.shape[0]
+        dtype = dtype_code(q.dtype)
+        pages = k_cache.shape[0]
+        if (tuple(q.shape) != (T, nq * hd) or tuple(out.shape) != (T, nq * hd) or tuple(k_cache.shape) != (pages, nkv, page_size, hd)
+                or k_cache.shape != v_cache.shape or mask.dim() != 2 or block_table.dim() != 2):
+            raise ShapeError(f"tree_attention: q {list(q.shape)}, out {list(out.shape)}, caches {list(k_cache.shape)} and "
+                             f"{list(v_cache.shape)}, mask {list(mask.shape)}, block table {list(block_table.shape)} with nq={nq} "
+                             f"nkv={nkv} hd={hd} page_size={page_size}")
+        if q.dtype != k_cache.dtype or q.dtype != v_cache.dtype or q.dtype != out.dtype:
+            raise ShapeError(f"tree_attention: q {q.dtype}, caches {k_cache.dtype} and {v_cache.dtype}, out {out.dtype}: one type")
+        self._ints("tree_attention", block_table=(block_table, (n, block_table.shape[1])), cu_q=(cu_q, (n + 1,)),
+                   kv_lens=(kv_lens, (n,)), mask=(mask, (T, mask.shape[1])))
+        if positions is not None:
+            self._ints("tree_attention", positions=(positions, (T,)))
+        if T == 0 or n == 0:
+            return
+        if max_q_len > 32 * mask.shape[1]:
+            raise ShapeError(f"tree_attention: {mask.shape[1]} words of a mask are too few for {max_q_len} tokens")
+        args = (_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out))
+        ints = (_ptr(block_table), C.c_int(block_table.shape[1]), _ptr(cu_q), _ptr(kv_lens), _ptr(mask), C.c_int(mask.shape[1]),
+                _ptr(positions))
+        self._here("tree_attention", q, k_cache, v_cache, out, block_table, cu_q, kv_lens, mask, positions)
+        sms = self.sm_count(q.device)
+        words = self._tree_words(dtype, nq, nkv, hd, page_size, max_q_len, sms)
+        # of this call alone: calls on several streams, and graphs recorded apart, share nothing
+        work = torch.empty(words, dtype=torch.float32, device=q.device)
+        self._check(self.lib.srlm_tree_attention(
+            *args, C.c_int(dtype), C.c_longlong(pages), *ints, C.c_int(n), C.c_int(T), C.c_int(nq), C.c_int(nkv), C.c_int(hd),
+            C.c_int(page_size), C.c_float(scale), C.c_int(window), C.c_int(max_q_len), _ptr(work), C.c_int(sms),
+            _ptr(self._gemm_state(q.device)[1]), _stream()), "tree_attention")
+        self.launches += 1               # the kernel that adds the shares
+
+    def _tree_words(self, *sizes) -> int:
+        words = self.__dict__.setdefault("_tree_work", {}).get(sizes)
+        if words is None:
+            self.lib.srlm_tree_attention_workspace.restype = C.c_longlong
+            words = self.lib.srlm_tree_attention_workspace(*(C.c_int(s) for s in sizes))
+            if words < 0:
+                raise ShapeError(f"tree_attention refused: {self.lib.srlm_last_error().decode(errors='replace')}")
+            self._tree_work[sizes] = words
+        return words
+
+    def accept_drafts(self, tokens, parents, targets, cu_q, path, count, next_token):
+        """Follows the model's own choice down each entry's tree of drafted tokens.
+
+        tokens, parents, targets int32 [T]: the drafted tokens, their parents as for ``draft_tree``, and the token that
+        the model chose behind each.  From the entry's token 0, which stands, the walk goes to the first child whose token
+        is the target of the token before, and on, until no child is, or path is full.  path int32 [n, room]: the
+        followed tokens' places in their entry, -1 behind them; count int32 [n]: how many; next_token int32 [n]: the target
+        of the last.  An entry without tokens has a count of 0 and -1."""
+        T, n = tokens.shape[0], count.shape[0]
+        if path.dim() != 2 or path.shape[1] < 1:
+            raise ShapeError(f"accept_drafts: path {list(path.shape)} has no room")
+        self._ints("accept_drafts", tokens=(tokens, (T,)), parents=(parents, (T,)), targets=(targets, (T,)), cu_q=(cu_q, (n + 1,)),
+                   path=(path, (n, path.shape[1])), count=(count, (n,)), next_token=(next_token, (n,)))
+        args = (_ptr(tokens), _ptr(parents), _ptr(targets), _ptr(cu_q))
+        outs = (_ptr(path), C.c_int(path.shape[1]), _ptr(count), _ptr(next_token))
+        self._here("accept_drafts", tokens, parents, targets, cu_q, path, count, next_token)
+        self._check(self.lib.srlm_accept_drafts(*args, C.c_int(n), C.c_int(T), *outs, _ptr(self._gemm_state(cu_q.device)[1]),
+                                                _stream()), "accept_drafts")
+
+    def _page_pool(self, what, pool):
+        """(slabs, pages) of a pool [.., pages, kv heads, page size, head size]: what stands before the pages are its slabs."""
+        if pool.dim() < 4 or pool.numel() == 0:
+            raise ShapeError(f"{what}: a pool is [.., pages, kv heads, page size, head size], got {list(pool.shape)}")
+        return pool.numel() // (pool.shape[-4] * pool.shape[-3] * pool.shape[-2] * pool.shape[-1]), pool.shape[-4]
+
+    def keep_drafts(self, pool, block_table, cu_q, kv_lens, path, count):
+        """Moves the accepted tokens' keys and values together, in every slab of ``pool`` [.., pages, kv heads, page
+        size, head size] (layers, keys and values): entry e's place kv_lens - its tokens + i takes what stands at
+        kv_lens - its tokens + path[e, i], for i < count[e]; other places keep what they hold.  block_table, cu_q and
+        kv_lens as for ``tree_attention``, path and count as ``accept_drafts`` leaves them: places that rise along the
+        path.  One that does not, or a page outside the pool, raises the error word and ends the entry's move there.  No
+        two entries hold a page in common among their own tokens'."""
+        slabs, pages = self._page_pool("keep_drafts", pool)
+        n = count.shape[0]
+        if path.dim() != 2 or path.shape[1] < 1 or block_table.dim() != 2:
+            raise ShapeError(f"keep_drafts: path {list(path.shape)}, block table {list(block_table.shape)}")
+        self._ints("keep_drafts", block_table=(block_table, (n, block_table.shape[1])), cu_q=(cu_q, (n + 1,)), kv_lens=(kv_lens, (n,)),
+                   path=(path, (n, path.shape[1])), count=(count, (n,)))
+        args = (_ptr(pool), C.c_longlong(slabs), C.c_longlong(pages), C.c_int(pool.shape[-3]), C.c_int(pool.shape[-2]),
+                C.c_longlong(pool.shape[-1] * pool.element_size()))
+        ints = (_ptr(block_table), C.c_int(block_table.shape[1]), _ptr(cu_q), _ptr(kv_lens), _ptr(path), C.c_int(path.shape[1]),
+                _ptr(count))
+        self._here("keep_drafts", pool, block_table, cu_q, kv_lens, path, count)
+        self._check(self.lib.srlm_keep_drafts(*args, *ints, C.c_int(n), _ptr(self._gemm_state(pool.device)[1]), _stream()),
+                    "keep_drafts")
+
+    def copy_pages(self, pool, src, dst):
+        """Page dst[i] takes what page src[i] holds, in every slab of ``pool`` [.., pages, kv heads, page size, head
+        size].  src and dst are page numbers on the host (the cache manager's); a page may be copied several times, none
+        is written twice, and none is both read and written."""
+        slabs, pages = self._page_pool("copy_pages", pool)
+        numbers = []
+        for x in (src, dst):
+            if isinstance(x, torch.Tensor) and x.is_cuda:
+                raise ShapeError("copy_pages: page numbers are the host's")
+            x = np.asarray(x)
+            if x.ndim != 1 or (x.size and x.dtype.kind not in "iu"):
+                raise ShapeError(f"copy_pages: page numbers are a list of whole numbers, got {x.dtype} {list(x.shape)}")
+            numbers.append(np.ascontiguousarray(x, dtype=np.int64))
+        if numbers[0].size != numbers[1].size:
+            raise ShapeError(f"copy_pages: {numbers[0].size} pages to {numbers[1].size}")
+        ptr = _ptr(pool)
+        self._here("copy_pages", pool)
+        self._check(self.lib.srlm_copy_pages(
+            ptr, C.c_longlong(slabs), C.c_longlong(pages), C.c_longlong(pool.shape[-3] * pool.shape[-2] * pool.shape[-1] * pool.element_size()),
+            C.c_void_p(numbers[0].ctypes.data), C.c_void_p(numbers[1].ctypes.data), C.c_int(numbers[0].size),
+            C.c_int(self.sm_count(pool.device)), _stream()), "copy_pages")
 
     # ---- blocks that norm on both sides of a sublayer --------------------------------
     def gated_postnorm_add(self, residual, sub, gate, gate_bias, post_w, eps, next_w=None, next_eps=0.0,
