@@ -259,6 +259,9 @@ struct Form {
 };
 Form simt_form(int hd, int sms);
 int run_simt(const Args& a, int dtype, int max_rows, int sms, cudaStream_t stream);
+bool mma_takes(int hd);                            // bfloat16
+Form mma_form(int hd, int max_rows, int sms);
+int run_mma(const Args& a, int max_rows, int sms, cudaStream_t stream);
 
 }  // namespace tree
 }  // namespace srlm
