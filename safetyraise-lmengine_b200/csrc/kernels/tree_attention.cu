@@ -5,10 +5,13 @@
 
 using namespace srlm;
 
-enum Kind { SIMT, MMA };
-static Kind kind_of(int dtype, int hd) { return dtype == DT_BF16 && tree::mma_takes(hd) ? MMA : SIMT; }
-static tree::Form form_of(int dtype, int hd, int max_rows, int sms) {
-  return kind_of(dtype, hd) == MMA ? tree::mma_form(hd, max_rows, sms) : tree::simt_form(hd, sms);
+enum Kind { SIMT, MMA, TCGEN05 };
+static Kind kind_of(int dtype, int hd, int page_size, int max_rows) {
+  if (dtype != DT_BF16 || !tree::mma_takes(hd)) return SIMT;
+  return max_rows > 16 && tree::tcgen05_takes(hd, page_size) ? TCGEN05 : MMA;
+}
+static tree::Form form_of(Kind kind, int hd, int max_rows, int sms) {
+  return kind == TCGEN05 ? tree::tcgen05_form(sms) : kind == MMA ? tree::mma_form(hd, max_rows, sms) : tree::simt_form(hd, sms);
 }
 
 // float32 words of workspace that srlm_tree_attention wants for these sizes, or -1 where it refuses them.
@@ -19,7 +22,8 @@ extern "C" long long srlm_tree_attention_workspace(int dtype, int nq, int nkv, i
            dtype, nq, nkv, hd, page_size, max_q_len);
     return -1;
   }
-  const tree::Form f = form_of(dtype, hd, max_q_len * (nq / nkv), sms);
+  const int max_rows = max_q_len * (nq / nkv);
+  const tree::Form f = form_of(kind_of(dtype, hd, page_size, max_rows), hd, max_rows, sms);
   return 2ll * f.blocks * f.rows * (hd + 2);
 }
 
@@ -34,16 +38,17 @@ extern "C" int srlm_tree_attention(const void* q, const void* k_cache, const voi
   if (words <= 0 || table_stride <= 0 || num_pages <= 0 || num_pages > 0x7fffffff || window < 0 || (window > 0 && !positions) || !work || !err_flag)
     return refuse(ST_BAD_SIZE, "tree_attention: words=%d table_stride=%d num_pages=%lld window=%d (a window needs the positions)", words,
                   table_stride, num_pages, window);
-  const tree::Form f = form_of(dtype, hd, max_q_len * (nq / nkv), sms);
+  const int max_rows = max_q_len * (nq / nkv);
+  const Kind kind = kind_of(dtype, hd, page_size, max_rows);
+  const tree::Form f = form_of(kind, hd, max_rows, sms);
   tree::Args a{q, k_cache, v_cache, out, block_table, table_stride, cu_q, kv_lens, mask, words, std::min(max_q_len, 32 * words), positions, n, T,
                nq, nkv, hd, page_size, (int)num_pages, scale * 1.4426950408889634f, window, 1, err_flag, work,
                work + 2ll * f.blocks * f.rows * hd};
-  const int max_rows = max_q_len * (nq / nkv);
-  if (kind_of(dtype, hd) == MMA) {
+  if (kind != SIMT) {
     if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) % 16)
       return refuse(ST_BAD_ALIGN, "tree_attention: bfloat16 tensors start on 16-byte boundaries");
     a.least_tiles = 2;
-    return tree::run_mma(a, max_rows, sms, stream);
+    return kind == TCGEN05 ? tree::run_tcgen05(a, max_rows, sms, stream) : tree::run_mma(a, max_rows, sms, stream);
   }
   a.least_tiles = 4;
   return tree::run_simt(a, dtype, max_rows, sms, stream);

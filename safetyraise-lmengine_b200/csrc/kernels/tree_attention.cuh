@@ -85,6 +85,14 @@ __device__ __forceinline__ long long warp_total(long long v) {
   return v;
 }
 
+// What a block does in one go: tiles of one unit.
+struct Piece {
+  Entry x;
+  int e, kvh, block;
+  int tile_lo, tile_hi;        // tiles of the entry's keys, from its first key on
+  bool begins, ends;           // the unit's first tile, its last one, are the piece's
+};
+
 // A block's share of the list.  Every warp that calls next() walks the same pieces.
 template <int ROWS, int KEYS>
 struct Walk {
@@ -93,9 +101,6 @@ struct Walk {
   int e;                       // entry of the tile `at`, whose list begins at `base`
   long long base;
   Entry x;
-  // the current piece
-  int kvh, block, tile_lo, tile_hi;          // tiles of the entry's keys, from its first key on
-  bool begins, ends;                         // the unit's first tile, its last one, are the piece's
 
   __device__ __forceinline__ long long weight(const Args& a, const Entry& y) const { return (long long)y.tiles * y.blocks * a.nkv; }
 
@@ -138,7 +143,7 @@ struct Walk {
     }
     x = entry_of<ROWS, KEYS>(a, e);
   }
-  __device__ __forceinline__ bool next(const Args& a) {
+  __device__ __forceinline__ bool next(const Args& a, Piece& p) {
     if (at >= end) return false;
     while (at - base >= weight(a, x)) {
       base += weight(a, x);
@@ -148,12 +153,14 @@ struct Walk {
     const int t = (int)(at - base - unit * x.tiles);
     const long long left = end - at;
     const int count = left < x.tiles - t ? (int)left : x.tiles - t;
-    kvh = (int)(unit / x.blocks);
-    block = (int)(unit % x.blocks);
-    tile_lo = x.first_tile + t;
-    tile_hi = tile_lo + count;
-    begins = t == 0;
-    ends = t + count == x.tiles;
+    p.x = x;
+    p.e = e;
+    p.kvh = (int)(unit / x.blocks);
+    p.block = (int)(unit % x.blocks);
+    p.tile_lo = x.first_tile + t;
+    p.tile_hi = p.tile_lo + count;
+    p.begins = t == 0;
+    p.ends = t + count == x.tiles;
     at += count;
     return true;
   }
@@ -202,10 +209,47 @@ __device__ __forceinline__ long long row_of_key(const Args& a, const int* table,
   return ((long long)page * a.nkv + kvh) * a.page_size + (j - pg * a.page_size);
 }
 
+// Values that are no numbers, in tiles where rows see different keys.  A product multiplies a value that a row does not see by
+// zero, which leaves nothing of a finite one alone: such values are taken out of the tile (take_loose: eight bfloat16 numbers;
+// whether there was one) and the rows that see them get them back as they are written (loose_values).
+__device__ __forceinline__ bool take_loose(uint4& v) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+  bool here = false;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const bool lo = (w[k] & 0x7f80u) == 0x7f80u, hi = (w[k] & 0x7f800000u) == 0x7f800000u;
+    if (lo) w[k] &= 0xffff0000u;
+    if (hi) w[k] &= 0xffffu;
+    here |= lo || hi;
+  }
+  return here;
+}
+
+// The sum of the non-finite values of dimension d that a row sees in the piece's masked tiles (all tiles are looked through: this is
+// for rows whose cache holds such values).
+template <int KEYS>
+__device__ __noinline__ float loose_values(const Args& a, int start, int kv_len, const int* table, int kvh, int token, int d, int tile_lo,
+                                           int tile_hi) {
+  float sum = 0.f;
+  const int lo = first_key_of(a, token, start);
+  const bf16* v = (const bf16*)a.v_cache;
+  for (int j0 = tile_lo * KEYS; j0 < tile_hi * KEYS && j0 < kv_len; j0 += 32) {
+    if (j0 / KEYS * KEYS + KEYS <= start && (a.window <= 0 || j0 / KEYS * KEYS >= kv_len - a.window)) continue;
+    uint32_t bits = seen_bits(a, a.mask + (size_t)token * a.words, j0, start, kv_len, lo);
+    while (bits) {
+      const int j = j0 + __ffs(bits) - 1;
+      bits &= bits - 1;
+      const float f = to_float(v[row_of_key(a, table, j, kvh) * a.hd + d]);
+      if (!isfinite(f)) sum += f;
+    }
+  }
+  return sum;
+}
+
 // Adds the slabs of the unit that begins in share blockIdx.x and goes on behind it, eight rows a block, a warp a row, a lane
 // every 32nd dimension: out = sum_z O_z 2^(m_z - M) / sum_z l_z 2^(m_z - M), M the largest reference of a slab that saw a key.
 template <typename T, int ROWS, int KEYS>
-__global__ void __launch_bounds__(256) tree_merge_kernel(const Args a, int blocks_there) {
+__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ Args a, int blocks_there) {
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -262,6 +306,9 @@ int run_simt(const Args& a, int dtype, int max_rows, int sms, cudaStream_t strea
 bool mma_takes(int hd);                            // bfloat16
 Form mma_form(int hd, int max_rows, int sms);
 int run_mma(const Args& a, int max_rows, int sms, cudaStream_t stream);
+bool tcgen05_takes(int hd, int page_size);         // bfloat16
+Form tcgen05_form(int sms);
+int run_tcgen05(const Args& a, int max_rows, int sms, cudaStream_t stream);
 
 }  // namespace tree
 }  // namespace srlm

@@ -25,27 +25,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ bool finite_pair(uint32_t w) { return (w & 0x7f80u) != 0x7f80u && (w & 0x7f800000u) != 0x7f800000u; }
-
-// The sum of the non-finite values of dimension d that a row sees in the piece's masked tiles (all tiles are looked through: this is
-// for rows whose cache holds such values).
-template <int KEYS>
-__device__ __noinline__ float loose_values(const Args& a, const Entry& x, const int* table, int kvh, int token, int d, int tile_lo, int tile_hi) {
-  float sum = 0.f;
-  const int lo = first_key_of(a, token, x.start);
-  const bf16* v = (const bf16*)a.v_cache;
-  for (int j0 = tile_lo * KEYS; j0 < tile_hi * KEYS && j0 < x.kv_len; j0 += 32) {
-    if (j0 / KEYS * KEYS + KEYS <= x.start && (a.window <= 0 || j0 / KEYS * KEYS >= x.kv_len - a.window)) continue;
-    uint32_t bits = seen_bits(a, a.mask + (size_t)token * a.words, j0, x.start, x.kv_len, lo);
-    while (bits) {
-      const int j = j0 + __ffs(bits) - 1;
-      bits &= bits - 1;
-      const float f = to_float(v[row_of_key(a, table, j, kvh) * a.hd + d]);
-      if (!isfinite(f)) sum += f;
-    }
-  }
-  return sum;
-}
 
 template <int HD_MAX, int KEY_WARPS, int STAGES>
 struct MmaForm {
@@ -58,7 +37,7 @@ struct MmaForm {
 };
 
 template <int HD_MAX, int KEY_WARPS, int STAGES>
-__global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const Args a) {
+__global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_constant__ Args a) {
   using Form = MmaForm<HD_MAX, KEY_WARPS, STAGES>;
   constexpr int ROWS = Form::ROWS, WK = M_KEYS / KEY_WARPS;      // keys of a warp in a tile
   constexpr int KS = HD_MAX / 16, NO = HD_MAX / 8, NS = WK / 8;
@@ -77,9 +56,10 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const Args a) {
   const int g = a.nq / a.nkv;
   pdl_wait();
   pdl_trigger();
-  Walk<ROWS, M_KEYS> w;
-  w.init(a, blockIdx.x, gridDim.x, blockIdx.x == 0);
-  while (w.next(a)) {
+  Walk<ROWS, M_KEYS> walk;
+  walk.init(a, blockIdx.x, gridDim.x, blockIdx.x == 0);
+  Piece w;
+  while (walk.next(a, w)) {
     const Entry& x = w.x;
     const int r0 = w.block * ROWS, rows = min(ROWS, x.q_len * g - r0), tiles = w.tile_hi - w.tile_lo;
     const int* table = a.block_table + (size_t)w.e * a.table_stride;
@@ -143,15 +123,7 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const Args a) {
         for (int i = tid; i < M_KEYS * chunks; i += M_THREADS) {
           uint4* p = reinterpret_cast<uint4*>(vt + i / chunks * ld + i % chunks * 8);
           uint4 v = *p;
-          uint32_t* wv = reinterpret_cast<uint32_t*>(&v);
-          bool here = false;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (!finite_pair(wv[k])) {
-              here = true;
-              if ((wv[k] & 0x7f80u) == 0x7f80u) wv[k] &= 0xffff0000u;
-              if ((wv[k] & 0x7f800000u) == 0x7f800000u) wv[k] &= 0xffffu;
-            }
+          const bool here = take_loose(v);
           if (here) {
             *p = v;
             loose = true;
@@ -263,8 +235,8 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const Args a) {
     auto put = [&](int row, int d, float v0, float v1, float inv) {
       if (loose) {
         const int t = x.q0 + (r0 + row) / g;
-        v0 += loose_values<M_KEYS>(a, x, table, w.kvh, t, d, w.tile_lo, w.tile_hi);
-        v1 += loose_values<M_KEYS>(a, x, table, w.kvh, t, d + 1, w.tile_lo, w.tile_hi);
+        v0 += loose_values<M_KEYS>(a, x.start, x.kv_len, table, w.kvh, t, d, w.tile_lo, w.tile_hi);
+        v1 += loose_values<M_KEYS>(a, x.start, x.kv_len, table, w.kvh, t, d + 1, w.tile_lo, w.tile_hi);
       }
       if (whole) {
         const int r = r0 + row;

@@ -21,7 +21,7 @@ __host__ __device__ inline int simt_ld(int hd) { return (hd + 3) / 4 * 4 + 4; } 
 static size_t simt_smem(int hd) { return sizeof(float) * ((size_t)(4 * S_KEYS + S_ROWS) * simt_ld(hd) + S_ROWS * S_KEYS); }
 
 template <typename T, int DIMS, bool COPY>
-__global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const Args a) {
+__global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const __grid_constant__ Args a) {
   extern __shared__ __align__(16) float tree_sh[];
   const int ld = simt_ld(a.hd), pieces = (a.hd + 3) / 4;
   float* k_sh = tree_sh;                           // [2][keys][ld]
@@ -35,9 +35,10 @@ __global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const Args a) {
   const int g = a.nq / a.nkv;
   pdl_wait();
   pdl_trigger();
-  Walk<S_ROWS, S_KEYS> w;
-  w.init(a, blockIdx.x, gridDim.x, blockIdx.x == 0);
-  while (w.next(a)) {
+  Walk<S_ROWS, S_KEYS> walk;
+  walk.init(a, blockIdx.x, gridDim.x, blockIdx.x == 0);
+  Piece w;
+  while (walk.next(a, w)) {
     const Entry& x = w.x;
     const int rows = min(S_ROWS, x.q_len * g - w.block * S_ROWS), r0 = w.block * S_ROWS;
     const int* table = a.block_table + (size_t)w.e * a.table_stride;

@@ -1,0 +1,474 @@
+// Attention for drafted tokens on the 5th-generation tensor cores: bfloat16 heads of 64 or 128, pages that a TMA box
+// covers.  What a row sees and how the work is divided: tree_attention.cuh.
+//
+// A unit is up to 128 rows (token x query head of a KV group), the M of one MMA, over tiles of 128 keys:
+//     S = Q . K^T      both in shared memory, K-major
+//     O += P . V       P in tensor memory (bfloat16, over the columns of S), V in shared memory, MN-major
+// Trees have few rows, so it is the keys that keep the tensor core busy: the piece's tiles go to two streams in turn, each
+// with an S and an O of its own in tensor memory (512 columns in all) and four softmax warps, a thread a row.  While one stream's
+// warps form the weights of a tile, the tensor core works for the other, and three stages of keys and values (six of heads of
+// 64) are in flight.  At the end of a piece the two streams' sums are joined as they are read from tensor memory (a warp reads
+// the same lanes of both; each stream's warps write half of the columns).
+// Warp 0 fetches (a lane a page box), one thread of warp 1 issues the MMAs, warps 2-5 and 6-9 are the streams' softmax.  A block
+// stays for all of its pieces: the fetches run ahead across them, and the block count is the SMs'.
+//
+// A weight is rounded to bfloat16 for the product with the values.  O is rescaled only when a row's maximum has grown by more
+// than 2^8: until then the old one stays the reference of the exponentials, and the division by the sum makes it exact.
+// Every wait is bounded; one that runs out raises the error word and ends the block's work.
+#include "attention_tcgen05.cuh"
+#include "tree_attention.cuh"
+
+namespace srlm {
+namespace tree {
+
+using namespace fmha;
+
+constexpr int T_ROWS = 128, T_KEYS = 128, T_THREADS = 320, T_SOFTMAX = 256;
+constexpr float T_RESCALE_ABOVE = 8.f;             // log2 of the growth of a row's maximum that O is rescaled for
+
+template <int HD>
+struct TmaForm {
+  static constexpr int TILE = T_KEYS * HD * 2;     // bytes of a tile of keys, values or rows
+  static constexpr int STAGES = HD == 128 ? 3 : 6;
+  static constexpr int SMEM = TILE * (1 + 2 * STAGES) + 1024 + (4 * STAGES + 7) * 8;
+};
+
+// The row's maximum over the keys that it sees (bits), and its weights exp2(S * scale - base) as bfloat16 pairs over the first 64
+// columns of S; the sum of the weights.
+__device__ __forceinline__ float row_max_seen(const Row& r, const uint32_t (&bits)[4]) {
+  float m[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+  auto part = [&](const uint32_t (&v)[32], uint32_t b) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) m[j & 3] = fmaxf(m[j & 3], (b >> j) & 1 ? __uint_as_float(v[j]) : -CUDART_INF_F);
+  };
+  part(r.a, bits[0]);
+  part(r.b, bits[1]);
+  part(r.c, bits[2]);
+  part(r.d, bits[3]);
+  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+__device__ __forceinline__ float row_exp_seen(uint32_t s_addr, const Row& r, float scale, float base, const uint32_t (&bits)[4]) {
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  auto part = [&](const uint32_t (&v)[32], uint32_t b, int c) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const float p0 = (b >> j) & 1 ? ex2(fmaf(__uint_as_float(v[j]), scale, -base)) : 0.f;
+      const float p1 = (b >> (j + 1)) & 1 ? ex2(fmaf(__uint_as_float(v[j + 1]), scale, -base)) : 0.f;
+      pk[j >> 1] = pack2(p0, p1);
+      sum[j & 2] += p0;
+      sum[(j & 2) + 1] += p1;
+    }
+    tmem_st16(s_addr + (c >> 1), pk);
+  };
+  part(r.a, bits[0], 0);
+  part(r.b, bits[1], 32);
+  part(r.c, bits[2], 64);
+  part(r.d, bits[3], 96);
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(T_THREADS, 1)
+tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a) {
+  using Form = TmaForm<HD>;
+  constexpr int TILE = Form::TILE, STAGES = Form::STAGES, CHUNKS = HD / 8;
+  extern __shared__ uint8_t tree_smem_raw[];
+  uint8_t* smem = tree_smem_raw + ((1024u - (s32(tree_smem_raw) & 1023u)) & 1023u);
+  uint8_t* q_t = smem;
+  uint8_t* k_t = q_t + TILE;                       // [STAGES]
+  uint8_t* v_t = k_t + STAGES * TILE;              // [STAGES]
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(v_t + STAGES * TILE);
+  uint64_t* k_empty = k_full + STAGES;
+  uint64_t* v_full = k_empty + STAGES;
+  uint64_t* v_empty = v_full + STAGES;
+  uint64_t* s_full = v_empty + STAGES;             // [2]: per stream
+  uint64_t* p_ready = s_full + 2;                  // [2]
+  uint64_t* o_done = p_ready + 2;                  // [2]
+  uint64_t* q_full = o_done + 2;
+  __shared__ Walk<T_ROWS, T_KEYS> walk_sh[3];
+  __shared__ uint32_t tmem_sh;
+  __shared__ int loose_sh, failed_sh;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_ready[i], 4);
+      mbar_init(&o_done[i], 1);
+    }
+    mbar_init(q_full, T_SOFTMAX / 32);
+    loose_sh = failed_sh = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&tmem_sh)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_sh;
+  pdl_wait();
+  pdl_trigger();
+
+  const int g = a.nq / a.nkv;
+  // the walk lies in shared memory between pieces, one for each role: its numbers would cost the softmax registers
+  using Walks = Walk<T_ROWS, T_KEYS>;
+  const int role = min(warp, 2);
+  Piece w;
+  {
+    Walks walk;
+    walk.init(a, blockIdx.x, gridDim.x, blockIdx.x == 0 && warp == 0);
+    if ((warp <= 2) && lane == 0) walk_sh[role] = walk;
+  }
+  __syncthreads();
+  // read: by every warp of the role; kept: by one of them once all have read (the softmax warps meet between two pieces)
+  auto next = [&] {
+    Walks walk = walk_sh[role];
+    const bool more = walk.next(a, w);
+    if (role < 2) {
+      __syncwarp();
+      if (lane == 0) walk_sh[role] = walk;
+      __syncwarp();
+    } else {
+      asm volatile("bar.sync 1, %0;" ::"n"(T_SOFTMAX) : "memory");
+      if (threadIdx.x == 64) walk_sh[2] = walk;
+    }
+    return more;
+  };
+  auto first_key = [&] { return a.window > 0 ? max(0, w.x.start - a.window + 1) : 0; };
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    const int ps = a.page_size, box_rows = ps < T_KEYS ? ps : T_KEYS, boxes = T_KEYS / box_rows;
+    int k = 0;                                     // tiles so far
+    bool ok = true;
+    int k_loads = 0, v_loads = 0;
+    while (ok && next()) {
+      const int* table = a.block_table + (size_t)w.e * a.table_stride;
+      const int first = first_key();
+      for (int t = w.tile_lo; t < w.tile_hi && ok; ++t, ++k) {
+        const int s = k % STAGES;
+        const uint32_t parity = ((k / STAGES) & 1) ^ 1;
+        int row = 0;
+        if (lane < boxes) {                        // the lanes' lookups of a tile overlap
+          const int key = t * T_KEYS + lane * box_rows, pg = key / ps;
+          int page = 0;
+          if (key < w.x.kv_len) {
+            page = table[pg];
+            if (page < 0 || page >= a.num_pages) {
+              if (key + box_rows > first) atomicExch(a.err_flag, ERR_PAGE);      // (pages behind a window are given back)
+              page = 0;
+            }
+          }
+          row = (page * a.nkv + w.kvh) * ps + (key - pg * ps);
+        }
+        auto load = [&](const CUtensorMap* map, uint8_t* tile, uint64_t* full) {
+          if (lane == 0) mbar_expect_tx(full, TILE);
+          __syncwarp();
+          if (lane < boxes) {
+#pragma unroll
+            for (int c = 0; c < HD; c += 64) tma_load_2d(tile + c * (T_KEYS * 2) + lane * box_rows * 128, map, full, c, row);
+          }
+        };
+        ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[s], parity, a.err_flag, 81));
+        if (!ok) break;
+        load(&map_k, k_t + s * TILE, &k_full[s]);
+        ++k_loads;
+        ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[s], parity, a.err_flag, 82));
+        if (!ok) break;
+        load(&map_v, v_t + s * TILE, &v_full[s]);
+        ++v_loads;
+      }
+    }
+    if (!ok)                                       // copies in flight end before the block does
+      for (int back = 1; back <= STAGES; ++back) {
+        if (back <= k_loads) mbar_wait(&k_full[(k_loads - back) % STAGES], ((k_loads - back) / STAGES) & 1, a.err_flag, 81);
+        if (back <= v_loads) mbar_wait(&v_full[(v_loads - back) % STAGES], ((v_loads - back) / STAGES) & 1, a.err_flag, 82);
+      }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    const uint32_t idesc_s = umma_idesc(T_KEYS, false), idesc_o = umma_idesc(HD, true);
+    // descriptors: the start address sits in the low bits, in units of 16 bytes, so a k-step is an addition
+    const uint64_t q_desc = umma_desc(s32(q_t), 0, 1024), k_desc = umma_desc(s32(k_t), 0, 1024);
+    const uint64_t v_desc = umma_desc(s32(v_t), T_KEYS * 128, 1024);
+    int k = 0, piece = 0;
+    uint32_t done[2] = {0, 0};                     // tiles of either stream so far
+    bool ok = true;
+    while (next()) {                            // (the whole warp walks, one lane issues)
+      if (lane == 0 && ok) {
+        const int tiles = w.tile_hi - w.tile_lo;
+        auto issue_s = [&](int t) {                // S_i = Q . K_t^T
+          const int s = (k + t) % STAGES, i = t & 1;
+          ok = ok && mbar_wait(&k_full[s], ((k + t) / STAGES) & 1, a.err_flag, 83);
+          if (!ok) return;
+          fence_after();
+          const uint64_t kd = k_desc + (uint64_t)(s * (TILE >> 4));
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint32_t off = ((ks >> 2) * (T_KEYS * 128) + (ks & 3) * 32) >> 4;      // panel, then 32 bytes a k-step
+            umma_bf16(tmem + i * 128, q_desc + off, kd + off, idesc_s, ks != 0);
+          }
+          umma_commit(&s_full[i]);
+          umma_commit(&k_empty[s]);
+        };
+        ok = mbar_wait(q_full, piece & 1, a.err_flag, 84);
+        if (ok) fence_after();
+        if (ok) issue_s(0);
+        if (ok && tiles > 1) issue_s(1);
+        for (int t = 0; t < tiles && ok; ++t) {
+          const int s = (k + t) % STAGES, i = t & 1;
+          ok = mbar_wait(&v_full[s], ((k + t) / STAGES) & 1, a.err_flag, 85) && mbar_wait(&p_ready[i], done[i] & 1, a.err_flag, 86);
+          if (!ok) break;
+          ++done[i];
+          fence_after();
+          const uint64_t vd = v_desc + (uint64_t)(s * (TILE >> 4));
+          const uint32_t d = tmem + 256 + i * 128, p = tmem + i * 128;
+#pragma unroll
+          for (int kk = 0; kk < T_KEYS / 16; ++kk)   // 16 keys: 8 columns of pairs, 2048 bytes of values
+            umma_bf16_ts(d, p + kk * 8, vd + kk * (2048 >> 4), idesc_o, t > 1 || kk > 0);
+          umma_commit(&o_done[i]);
+          umma_commit(&v_empty[s]);
+          if (t + 2 < tiles) issue_s(t + 2);
+        }
+        k += tiles;
+        ++piece;
+      }
+      __syncwarp();
+    }
+  } else {
+    // ---------------- softmax: a thread a row ----------------
+    const int i = (warp - 2) >> 2, ew = warp & 3, row = ew * 32 + lane, st = threadIdx.x - 64;
+    const uint32_t lane_addr = (uint32_t)(ew * 32) << 16;
+    const uint32_t s_addr = tmem + i * 128 + lane_addr, o_addr = tmem + 256 + i * 128 + lane_addr;
+    auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(T_SOFTMAX) : "memory"); };      // both streams
+    uint32_t done = 0;                             // tiles of this stream so far
+    int k = 0;                                     // tiles of the block so far
+    bool ok = true;
+    while (next()) {
+      const Entry& x = w.x;
+      const int rows_total = x.q_len * g, r0 = w.block * T_ROWS, rows = min(T_ROWS, rows_total - r0), tiles = w.tile_hi - w.tile_lo;
+      const int first = first_key();
+      // the rows -> shared memory, swizzled (zeros behind the last), eight loads of a thread in flight; the products that read the last
+      // piece's are done (their tiles were waited for)
+      const bf16* q = (const bf16*)a.q;
+      constexpr int QB = 8;
+#pragma unroll 1
+      for (int base = st; base < T_ROWS * CHUNKS; base += T_SOFTMAX * QB) {
+        uint4 v[QB];
+#pragma unroll
+        for (int j = 0; j < QB; ++j) {
+          const int idx = base + j * T_SOFTMAX, rr = idx / CHUNKS, c = idx % CHUNKS, r = r0 + rr;
+          v[j] = make_uint4(0, 0, 0, 0);
+          if (rr < rows) v[j] = __ldg(reinterpret_cast<const uint4*>(q + ((size_t)(x.q0 + r / g) * a.nq + w.kvh * g + r % g) * HD + c * 8));
+        }
+#pragma unroll
+        for (int j = 0; j < QB; ++j) {
+          const int idx = base + j * T_SOFTMAX, rr = idx / CHUNKS, c = idx % CHUNKS;
+          if (rr < T_ROWS)
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(tile_addr(s32(q_t), rr, c)), "r"(v[j].x), "r"(v[j].y), "r"(v[j].z),
+                         "r"(v[j].w) : "memory");
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+
+      const int r = min(r0 + row, rows_total - 1), token = x.q0 + r / g;
+      const int lo = first_key_of(a, token, x.start);
+      const int* row_mask = a.mask + (size_t)token * a.words;
+      const bool live = ew * 32 < rows;            // some row of the warp is one
+      float m_run = -CUDART_INF_F, l_run = 0.f;
+      bool any = false;
+      for (int t = i; t < tiles && ok; t += 2, ++done, any = true) {
+        const int j0 = (w.tile_lo + t) * T_KEYS;
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[i], done & 1, a.err_flag, 87));
+        if (!ok) break;
+        fence_after();
+        // every row sees every key of a tile between the window's last edge and the drafted tokens
+        const bool plain = j0 + T_KEYS <= x.start && (a.window <= 0 || j0 >= x.kv_len - a.window);
+        if (!plain) {
+          // values of no key of the entry become zeros, and those that are no numbers are taken out
+          const int s = (k + t) % STAGES;
+          ok = __all_sync(0xffffffffu, mbar_wait(&v_full[s], ((k + t) / STAGES) & 1, a.err_flag, 88));
+          if (!ok) break;
+          const uint32_t vt = s32(v_t + s * TILE);
+          bool loose = false;
+          for (int idx = ew * 32 + lane; idx < T_KEYS * CHUNKS; idx += 128) {
+            const int key = idx / CHUNKS;
+            const uint32_t at = tile_addr(vt, key, idx % CHUNKS);
+            uint4 v;
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+            bool change;
+            if (j0 + key < first || j0 + key >= x.kv_len) {
+              v = make_uint4(0, 0, 0, 0);
+              change = true;
+            } else {
+              change = take_loose(v);
+              loose |= change;
+            }
+            if (change) asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+          }
+          if (loose) loose_sh = 1;
+          fence_async_smem();
+        }
+        if (live) {
+          Row srow;
+          load_row(s_addr, srow);
+          uint32_t bits[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+          if (!plain)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) bits[c] = seen_bits(a, row_mask, j0 + 32 * c, x.start, x.kv_len, lo);
+          const float mx = (plain ? row_max<false>(srow, 0, T_KEYS) : row_max_seen(srow, bits)) * a.scale_log2;
+          const bool grow = mx > m_run + T_RESCALE_ABOVE || m_run == -CUDART_INF_F;
+          const float m_new = grow ? fmaxf(mx, m_run) : m_run;
+          if (any && __any_sync(0xffffffffu, m_new != m_run)) {
+            const float alpha = m_new == m_run ? 1.f : ex2(m_run - m_new);      // (from -inf: 0)
+            ok = __all_sync(0xffffffffu, mbar_wait(&o_done[i], (done - 1) & 1, a.err_flag, 89));         // the tile before is in O
+            fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) {
+              uint32_t v[16];
+              tmem_ld16(o_addr + c, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
+              tmem_st16(o_addr + c, v);
+            }
+            l_run *= alpha;
+          }
+          m_run = m_new;
+          const float base = m_run == -CUDART_INF_F ? 0.f : m_run;
+          l_run += plain ? row_exp<false>(s_addr, srow, a.scale_log2, base, 0, T_KEYS) : row_exp_seen(s_addr, srow, a.scale_log2, base, bits);
+          tmem_wait_st();
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[i]);
+      }
+      if (ok && any) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[i], (done - 1) & 1, a.err_flag, 90));
+      k += tiles;
+      if (!ok) failed_sh = 1;
+      if (ok && any && live) {                     // the row's reference and sum over the first columns of S, whose weights are used up
+        uint32_t ml[16] = {__float_as_uint(m_run), __float_as_uint(l_run)};
+        tmem_st16(s_addr, ml);
+        tmem_wait_st();
+      }
+      fence_before();
+      meet();
+      fence_after();
+      ok = ok && !failed_sh;
+      if (ok && live) {
+        // both streams' sums of the row, half of the columns each
+        const bool two = tiles > 1;
+        float2 s0, s1 = make_float2(0.f, 0.f);
+        {
+          uint32_t ml[16];
+          tmem_ld16(tmem + lane_addr, ml);
+          tmem_wait_ld();
+          s0 = make_float2(__uint_as_float(ml[0]), __uint_as_float(ml[1]));
+          if (two) {
+            tmem_ld16(tmem + 128 + lane_addr, ml);
+            tmem_wait_ld();
+            s1 = make_float2(__uint_as_float(ml[0]), __uint_as_float(ml[1]));
+          }
+        }
+        const float M = two ? fmaxf(s0.x, s1.x) : s0.x, mb = M == -CUDART_INF_F ? 0.f : M;
+        const float f0 = ex2(s0.x - mb), f1 = two ? ex2(s1.x - mb) : 0.f;
+        const float L = two ? f0 * s0.y + f1 * s1.y : f0 * s0.y;
+        const bool mine = row < rows, whole = w.begins && w.ends;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const size_t slab = slab_of(blockIdx.x, w.begins) * T_ROWS + row;
+        if (!whole && mine && i == 0) *reinterpret_cast<float2*>(a.part_ml + slab * 2) = make_float2(M, L);
+        bf16* dst = (bf16*)a.out + ((size_t)token * a.nq + w.kvh * g + r % g) * HD;
+        const uint32_t both = tmem + 256 + lane_addr;
+#pragma unroll 1
+        for (int c = i * (HD / 2); c < (i + 1) * (HD / 2); c += 16) {
+          uint32_t u[16], v[16];
+          tmem_ld16(both + c, u);
+          if (two) tmem_ld16(both + 128 + c, v);
+          tmem_wait_ld();
+          float o[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            o[j] = f0 * __uint_as_float(u[j]);
+            if (two) o[j] = fmaf(f1, __uint_as_float(v[j]), o[j]);
+          }
+          if (loose_sh && mine)
+#pragma unroll 1
+            for (int j = 0; j < 16; ++j) {
+              const float more = loose_values<T_KEYS>(a, x.start, x.kv_len, a.block_table + (size_t)w.e * a.table_stride, w.kvh, token, c + j, w.tile_lo, w.tile_hi);
+#pragma unroll
+              for (int n = 0; n < 16; ++n) o[n] += n == j ? more : 0.f;
+            }
+          if (mine && whole) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+              *reinterpret_cast<uint4*>(dst + c + 8 * n) =
+                  make_uint4(pack2(o[8 * n] * inv, o[8 * n + 1] * inv), pack2(o[8 * n + 2] * inv, o[8 * n + 3] * inv),
+                             pack2(o[8 * n + 4] * inv, o[8 * n + 5] * inv), pack2(o[8 * n + 6] * inv, o[8 * n + 7] * inv));
+          } else if (mine) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+              *reinterpret_cast<float4*>(a.part_o + slab * HD + c + 4 * n) = make_float4(o[4 * n], o[4 * n + 1], o[4 * n + 2], o[4 * n + 3]);
+          }
+        }
+        fence_before();
+      }
+      meet();                                      // O, S and the rows are free
+      if (st == 0) loose_sh = 0;                   // (read before the meeting, set behind the next piece's first tile)
+      if (!ok) break;
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// ---------------------------------------------------------------------------
+static bool tensor_map(CUtensorMap* out, const void* ptr, long long rows, int hd, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)hd * 2};
+  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  cuuint32_t elem[2] = {1, 1};
+  return fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool tcgen05_takes(int hd, int page_size) {
+  return (hd == 64 || hd == 128) && (page_size == 8 || page_size == 16 || page_size == 32 || page_size == 64 ||
+                                     (page_size > 0 && page_size % T_KEYS == 0));
+}
+Form tcgen05_form(int sms) { return Form{sms, T_ROWS}; }
+
+template <int HD>
+static int run_form(const Args& a, int max_rows, int sms, cudaStream_t stream) {
+  const int box_rows = min(a.page_size, T_KEYS);
+  const long long rows = (long long)a.num_pages * a.nkv * a.page_size;
+  CUtensorMap mk, mv;
+  if (rows > 0x7fffffff || !tensor_map(&mk, a.k_cache, rows, HD, box_rows) || !tensor_map(&mv, a.v_cache, rows, HD, box_rows))
+    return refuse(ST_BAD_SIZE, "tree_attention: the caches of %lld rows of %d cannot be mapped", rows, HD);
+  const cudaError_t e = cudaFuncSetAttribute(tree_tcgen05_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, TmaForm<HD>::SMEM);
+  if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", TmaForm<HD>::SMEM);
+  launch_pdl(tree_tcgen05_kernel<HD>, dim3(sms), dim3(T_THREADS), TmaForm<HD>::SMEM, stream, mk, mv, a);
+  launch_pdl(tree_merge_kernel<bf16, T_ROWS, T_KEYS>, dim3(sms, (min(max_rows, T_ROWS) + 7) / 8), dim3(256), 0, stream, a, sms);
+  return launched();
+}
+int run_tcgen05(const Args& a, int max_rows, int sms, cudaStream_t stream) {
+  return a.hd == 64 ? run_form<64>(a, max_rows, sms, stream) : run_form<128>(a, max_rows, sms, stream);
+}
+
+}  // namespace tree
+}  // namespace srlm
