@@ -35,12 +35,18 @@ extern "C" int srlm_tree_attention(const void* q, const void* k_cache, const voi
                                    int window, int max_q_len, float* work, int sms, int* err_flag, cudaStream_t stream) {
   if (n <= 0 || T <= 0) return ST_OK;
   if (srlm_tree_attention_workspace(dtype, nq, nkv, hd, page_size, max_q_len, sms) < 0) return ST_BAD_SIZE;
-  if (words <= 0 || table_stride <= 0 || num_pages <= 0 || num_pages > 0x7fffffff || window < 0 || (window > 0 && !positions) || !work || !err_flag)
-    return refuse(ST_BAD_SIZE, "tree_attention: words=%d table_stride=%d num_pages=%lld window=%d (a window needs the positions)", words,
-                  table_stride, num_pages, window);
+  if (words <= 0 || table_stride <= 0 || num_pages <= 0 || num_pages > 0x7fffffff || window < 0 || (window > 0 && !positions) || !(scale > 0.f) || !work ||
+      !err_flag)
+    return refuse(ST_BAD_SIZE, "tree_attention: words=%d table_stride=%d num_pages=%lld window=%d scale=%g (a window needs the positions, a "
+                  "scale is positive)", words, table_stride, num_pages, window, (double)scale);
   const int max_rows = max_q_len * (nq / nkv);
   const Kind kind = kind_of(dtype, hd, page_size, max_rows);
   const tree::Form f = form_of(kind, hd, max_rows, sms);
+  // the list of all units' tiles is counted in 31 bits
+  const double units = (double)n * nkv * ((double)max_q_len * (nq / nkv) / f.rows + 1), tiles = (double)table_stride * page_size / f.keys + 1;
+  if (units * tiles > 2147483647.0)
+    return refuse(ST_BAD_SIZE, "tree_attention: %d entries of up to %d tokens and %d pages are more work than a call takes", n, max_q_len,
+                  table_stride);
   tree::Args a{q, k_cache, v_cache, out, block_table, table_stride, cu_q, kv_lens, mask, words, std::min(max_q_len, 32 * words), positions, n, T,
                nq, nkv, hd, page_size, (int)num_pages, scale * 1.4426950408889634f, window, 1, err_flag, work,
                work + 2ll * f.blocks * f.rows * hd};

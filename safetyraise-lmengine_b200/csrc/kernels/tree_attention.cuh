@@ -46,7 +46,7 @@ struct Args {
   int window;
   int least_tiles;           // a block takes at least so many tiles
   int* err_flag;
-  float* part_o;             // [2 C][ROWS][hd]
+  float* part_o;             // slabs [2 C][hd][ROWS]: neighbouring rows side by side, as the threads that write and read them are
   float* part_ml;            // [2 C][ROWS][2]: reference maximum (log2 units), sum of weights
 };
 
@@ -79,12 +79,6 @@ __device__ __forceinline__ Entry entry_of(const Args& a, int e, bool flag = fals
   return x;
 }
 
-__device__ __forceinline__ long long warp_total(long long v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 // What a block does in one go: tiles of one unit.
 struct Piece {
   Entry x;
@@ -93,43 +87,49 @@ struct Piece {
   bool begins, ends;           // the unit's first tile, its last one, are the piece's
 };
 
-// A block's share of the list.  Every warp that calls next() walks the same pieces.
+// A block's share of the list.  Every warp that calls next() walks the same pieces.  (A list is shorter than 2^31: the entry
+// point sees to it.)
 template <int ROWS, int KEYS>
 struct Walk {
-  long long total, at, end;    // tiles of the list; the next one and the share's end
-  int blocks;                  // blocks that have a share
-  int e;                       // entry of the tile `at`, whose list begins at `base`
-  long long base;
+  int at, end;                 // the next tile and the share's end
+  int blocks, each, more;      // blocks that have a share; of `each` tiles, the first `more` of them of one more
+  int e, base;                 // entry of the tile `at`, whose list begins at `base`
   Entry x;
 
-  __device__ __forceinline__ long long weight(const Args& a, const Entry& y) const { return (long long)y.tiles * y.blocks * a.nkv; }
+  __device__ __forceinline__ int weight(const Args& a, const Entry& y) const { return y.tiles * y.blocks * a.nkv; }
+  __device__ __forceinline__ int first_of(int share) const { return share * each + min(share, more); }
+  // the share that holds the tile `pos`
+  __device__ __forceinline__ int share_of(int pos) const {
+    const int longer = more * (each + 1);
+    return pos < longer ? pos / (each + 1) : more + (pos - longer) / each;
+  }
 
-  // All lanes of a warp.  share: which of `blocks_there`; the entries' tiles are counted by the warp, 32 entries a turn.
+  // All lanes of a warp.  share: which of `blocks_there`; the entries' tiles are counted by the warp, 32 entries a turn.  LAST: stands
+  // at the share's last tile instead of its first.
+  template <bool LAST = false>
   __device__ __forceinline__ void init(const Args& a, int share, int blocks_there, bool flag) {
     const int lane = threadIdx.x & 31;
-    total = 0;
-    for (int e0 = 0; e0 < a.n; e0 += 32)
-      total += warp_total(e0 + lane < a.n ? weight(a, entry_of<ROWS, KEYS>(a, e0 + lane, flag)) : 0);
-    const long long most = (total + a.least_tiles - 1) / a.least_tiles;
-    blocks = (int)(most < blocks_there ? most : blocks_there);
-    at = end = base = 0;
-    e = 0;
-    if (share < blocks) {
-      at = share * total / blocks;
-      end = (share + 1ll) * total / blocks;
-    }
-    if (at < end) seek(a, at);
-  }
-  // the entry that holds the tile `pos`
-  __device__ __forceinline__ void seek(const Args& a, long long pos) {
-    const int lane = threadIdx.x & 31;
-    long long before = 0;
+    int w = 0, total = 0;
     for (int e0 = 0; e0 < a.n; e0 += 32) {
-      const long long w = e0 + lane < a.n ? weight(a, entry_of<ROWS, KEYS>(a, e0 + lane)) : 0;
-      long long upto = w;
+      w = e0 + lane < a.n ? weight(a, entry_of<ROWS, KEYS>(a, e0 + lane, flag)) : 0;
+      total += __reduce_add_sync(0xffffffffu, w);
+    }
+    blocks = min((total + a.least_tiles - 1) / a.least_tiles, blocks_there);
+    at = end = base = e = each = more = 0;
+    if (share >= blocks) return;
+    each = total / blocks;
+    more = total - each * blocks;
+    at = first_of(share);
+    end = first_of(share + 1);
+    // the entry that holds the tile
+    const int pos = LAST ? end - 1 : at;
+    int before = 0;
+    for (int e0 = 0; e0 < a.n; e0 += 32) {
+      if (a.n > 32) w = e0 + lane < a.n ? weight(a, entry_of<ROWS, KEYS>(a, e0 + lane)) : 0;
+      int upto = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
       }
       const unsigned beyond = __ballot_sync(0xffffffffu, before + upto > pos);
@@ -149,14 +149,11 @@ struct Walk {
       base += weight(a, x);
       x = entry_of<ROWS, KEYS>(a, ++e);          // (at is below the total: such an entry is there)
     }
-    const long long unit = (at - base) / x.tiles;
-    const int t = (int)(at - base - unit * x.tiles);
-    const long long left = end - at;
-    const int count = left < x.tiles - t ? (int)left : x.tiles - t;
+    const int unit = (at - base) / x.tiles, t = at - base - unit * x.tiles, count = min(end - at, x.tiles - t);
     p.x = x;
     p.e = e;
-    p.kvh = (int)(unit / x.blocks);
-    p.block = (int)(unit % x.blocks);
+    p.kvh = unit / x.blocks;
+    p.block = unit - p.kvh * x.blocks;
     p.tile_lo = x.first_tile + t;
     p.tile_hi = p.tile_lo + count;
     p.begins = t == 0;
@@ -169,28 +166,32 @@ struct Walk {
 // The slab of a piece that is not a whole unit.
 __device__ __forceinline__ size_t slab_of(int share, bool begins) { return 2 * (size_t)share + (begins ? 1 : 0); }
 
-// Which of the 32 keys from j0 on a row sees, as bits.  row_mask: the row's token's words; lo: its first committed key.
-__device__ __forceinline__ uint32_t seen_bits(const Args& a, const int* row_mask, int j0, int start, int kv_len, int lo) {
-  uint32_t bits = 0;
-  if (j0 < start) {                               // committed keys [max(lo, j0), min(start, j0 + 32))
-    const int from = max(lo - j0, 0), to = min(start - j0, 32);
-    if (from < to) bits = (to >= 32 ? 0xffffffffu : (1u << to) - 1u) & ~(from > 0 ? (1u << from) - 1u : 0u);
+// Which keys of a tile a row sees, as bits, 32 a word.  words(): the part of the row's mask that the tile needs, N + 1 loads in
+// flight at once, which may be made ahead; bits(): the tile's keys from j0 on.
+template <int N>
+struct Sight {
+  uint32_t w[N + 1];
+  __device__ __forceinline__ void words(const Args& a, int token, int j0, int start) {
+    const int* row_mask = a.mask + (size_t)token * a.words;
+    const int first = (j0 - start) >> 5;                         // (rounded down: below zero the tile begins in front of the tokens)
+#pragma unroll
+    for (int i = 0; i <= N; ++i) w[i] = first + i >= 0 && first + i < a.words ? (uint32_t)row_mask[first + i] : 0u;
   }
-  const int k = j0 - start;                       // drafted tokens k, k + 1, ...
-  if (k > -32) {
-    uint32_t own;
-    if (k < 0) {
-      own = (uint32_t)row_mask[0] << -k;
-    } else {
-      const int w = k >> 5;
-      const uint32_t low = w < a.words ? (uint32_t)row_mask[w] : 0u, high = w + 1 < a.words ? (uint32_t)row_mask[w + 1] : 0u;
-      own = __funnelshift_r(low, high, k & 31);
+  // lo: the row's first committed key
+  __device__ __forceinline__ void bits(uint32_t (&out)[N], int j0, int start, int kv_len, int lo) const {
+    const int shift = (j0 - start) & 31;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int j = j0 + 32 * i;
+      uint32_t own = __funnelshift_r(w[i], w[i + 1], shift);     // drafted tokens j - start, ...
+      const int to = kv_len - j;                                 // bits of tokens that the entry does not have are nobody's
+      own = to <= 0 ? 0u : to >= 32 ? own : own & ((1u << to) - 1u);
+      const int from = max(lo - j, 0), upto = min(start - j, 32);      // committed keys [max(lo, j), min(start, j + 32))
+      if (from < upto) own |= (upto >= 32 ? 0xffffffffu : (1u << upto) - 1u) & ~((1u << from) - 1u);
+      out[i] = own;
     }
-    const int to = min(kv_len - j0, 32);          // bits of tokens that the entry does not have are nobody's
-    bits |= to <= 0 ? 0u : to >= 32 ? own : own & ((1u << to) - 1u);
   }
-  return bits;
-}
+};
 
 // The first committed key that a token's window leaves it (a position in front of the token's own place counts as that place).
 __device__ __forceinline__ int first_key_of(const Args& a, int token, int start) {
@@ -235,10 +236,13 @@ __device__ __noinline__ float loose_values(const Args& a, int start, int kv_len,
   const bf16* v = (const bf16*)a.v_cache;
   for (int j0 = tile_lo * KEYS; j0 < tile_hi * KEYS && j0 < kv_len; j0 += 32) {
     if (j0 / KEYS * KEYS + KEYS <= start && (a.window <= 0 || j0 / KEYS * KEYS >= kv_len - a.window)) continue;
-    uint32_t bits = seen_bits(a, a.mask + (size_t)token * a.words, j0, start, kv_len, lo);
-    while (bits) {
-      const int j = j0 + __ffs(bits) - 1;
-      bits &= bits - 1;
+    Sight<1> sight;
+    uint32_t bits[1];
+    sight.words(a, token, j0, start);
+    sight.bits(bits, j0, start, kv_len, lo);
+    while (bits[0]) {
+      const int j = j0 + __ffs(bits[0]) - 1;
+      bits[0] &= bits[0] - 1;
       const float f = to_float(v[row_of_key(a, table, j, kvh) * a.hd + d]);
       if (!isfinite(f)) sum += f;
     }
@@ -246,60 +250,77 @@ __device__ __noinline__ float loose_values(const Args& a, int start, int kv_len,
   return sum;
 }
 
-// Adds the slabs of the unit that begins in share blockIdx.x and goes on behind it, eight rows a block, a warp a row, a lane
-// every 32nd dimension: out = sum_z O_z 2^(m_z - M) / sum_z l_z 2^(m_z - M), M the largest reference of a slab that saw a key.
+// Adds the slabs of the unit that begins in share blockIdx.x and goes on behind it: out = sum_z O_z 2^(m_z - M) / sum_z l_z
+// 2^(m_z - M), M the largest reference of a slab that saw a key.  A lane has a row and MERGE_DIMS of its dimensions (a warp of fewer
+// rows than lanes several such runs); blockIdx.y and z run over groups of MERGE_WARPS runs and 32 rows.  The division of the work is
+// found while the kernel ahead still runs (its own blocks have waited for all that it reads of the lengths).
+constexpr int MERGE_WARPS = 4, MERGE_DIMS = 8;
+
 template <typename T, int ROWS, int KEYS>
-__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ Args a, int blocks_there) {
+__global__ void __launch_bounds__(32 * MERGE_WARPS) tree_merge_kernel(const __grid_constant__ Args a, int blocks_there) {
+  constexpr int RL = ROWS < 32 ? ROWS : 32, RUNS = 32 / RL;            // rows, runs of a warp
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int share = blockIdx.x, row = blockIdx.z * RL + lane % RL;
+  const int d0 = ((blockIdx.y * MERGE_WARPS + warp) * RUNS + lane / RL) * MERGE_DIMS;
+  Walk<ROWS, KEYS> w;
+  w.template init<true>(a, share, blocks_there, false);
+  bool mine = w.at < w.end;
+  int share_last = 0;
+  T* dst = nullptr;
+  if (mine) {
+    const int unit = (w.end - 1 - w.base) / w.x.tiles, from = w.base + unit * w.x.tiles, to = from + w.x.tiles;
+    const int kvh = unit / w.x.blocks, g = a.nq / a.nkv, r = (unit - kvh * w.x.blocks) * ROWS + row;
+    // else another share's unit, or a whole one, or no row
+    mine = from >= w.at && to > w.end && row < ROWS && r < w.x.q_len * g && d0 < a.hd;
+    if (mine) {
+      share_last = w.share_of(to - 1);
+      dst = (T*)a.out + ((size_t)(w.x.q0 + r / g) * a.nq + kvh * g + r % g) * a.hd + d0;
+    }
+  }
   pdl_wait();
   pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int share = blockIdx.x;
-  Walk<ROWS, KEYS> w;
-  w.init(a, share, blocks_there, false);
-  if (w.at >= w.end) return;
-  const long long lo = w.at, last = w.end - 1;
-  w.seek(a, last);
-  const long long unit = (last - w.base) / w.x.tiles, from = w.base + unit * w.x.tiles, to = from + w.x.tiles;
-  if (from < lo || to <= w.end) return;                        // another share's unit, or a whole one
-  const int kvh = (int)(unit / w.x.blocks), block = (int)(unit % w.x.blocks), g = a.nq / a.nkv;
-  const int row = blockIdx.y * 8 + warp, r = block * ROWS + row;
-  if (row >= ROWS || r >= w.x.q_len * g) return;
-  const int share_last = (int)((to * w.blocks - 1) / w.total);  // whose tiles hold the unit's last one
+  if (!mine) return;
+  const int slabs = share_last - share + 1;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row;
+  auto slab = [&](int z) { return slab_of(share + z, z == 0); };
   float M = -CUDART_INF_F;
-  for (int s = share + lane; s <= share_last; s += 32) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (slab_of(s, s == share) * ROWS + row) * 2);
-    if (ml.y > 0.f) M = fmaxf(M, ml.x);
+#pragma unroll 4
+  for (int z = 0; z < slabs; ++z) {
+    const float2 v = ml[slab(z) * ROWS];
+    if (v.y > 0.f) M = fmaxf(M, v.x);
   }
-  M = warp_max(M);
-  constexpr int MOST = 8;                                       // dimensions of a lane: heads up to 256
-  float acc[MOST], L = 0.f;
+  float acc[MERGE_DIMS], L = 0.f;
 #pragma unroll
-  for (int i = 0; i < MOST; ++i) acc[i] = 0.f;
-  for (int s = share; s <= share_last; ++s) {
-    const size_t at = slab_of(s, s == share) * ROWS + row;
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
-    if (!(ml.y > 0.f)) {
-      if (ml.y != ml.y) L = ml.y;                               // a score that was no number
-      continue;
-    }
-    const float wz = exp2f(ml.x - M);
-    L += wz * ml.y;
-    if (wz > 0.f) {
+  for (int i = 0; i < MERGE_DIMS; ++i) acc[i] = 0.f;
+  const int dims = min(MERGE_DIMS, a.hd - d0);
+#pragma unroll 2
+  for (int z = 0; z < slabs; ++z) {
+    const float2 v = ml[slab(z) * ROWS];
+    const float* src = a.part_o + (slab(z) * a.hd + d0) * ROWS + row;
+    float o[MERGE_DIMS];
 #pragma unroll
-      for (int i = 0; i < MOST; ++i)
-        if (lane + 32 * i < a.hd) acc[i] += wz * a.part_o[at * a.hd + lane + 32 * i];
-    }
+    for (int i = 0; i < MERGE_DIMS; ++i) o[i] = i < dims ? src[i * ROWS] : 0.f;
+    const float f = v.y > 0.f ? exp2f(v.x - M) : 0.f;
+    L += v.y != v.y ? v.y : f * v.y;                                   // (a score that was no number makes the row none)
+    if (f > 0.f)                                                       // (a slab of no key holds nothing)
+#pragma unroll
+      for (int i = 0; i < MERGE_DIMS; ++i) acc[i] += f * o[i];
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  T* dst = (T*)a.out + ((size_t)(w.x.q0 + r / g) * a.nq + kvh * g + r % g) * a.hd;
 #pragma unroll
-  for (int i = 0; i < MOST; ++i)
-    if (lane + 32 * i < a.hd) dst[lane + 32 * i] = from_float<T>(acc[i] * inv);
+  for (int i = 0; i < MERGE_DIMS; ++i)
+    if (i < dims) dst[i] = from_float<T>(acc[i] * inv);
+}
+template <typename T, int ROWS, int KEYS>
+inline void launch_merge(const Args& a, int blocks, int max_rows, cudaStream_t stream) {
+  constexpr int RL = ROWS < 32 ? ROWS : 32, SPAN = 32 / RL * MERGE_WARPS * MERGE_DIMS;
+  launch_pdl(tree_merge_kernel<T, ROWS, KEYS>, dim3(blocks, (a.hd + SPAN - 1) / SPAN, ((max_rows < ROWS ? max_rows : ROWS) + RL - 1) / RL),
+             dim3(32 * MERGE_WARPS), 0, stream, a, blocks);
 }
 
-// The forms.  Each gives its blocks (C) and rows of a unit, which size the slabs.
+// The forms.  Each gives its blocks (C) and the rows of a unit, which size the slabs, and the keys of a tile.
 struct Form {
-  int blocks, rows;
+  int blocks, rows, keys;
 };
 Form simt_form(int hd, int sms);
 int run_simt(const Args& a, int dtype, int max_rows, int sms, cudaStream_t stream);

@@ -116,6 +116,11 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
       locate(t + STAGES);
       const int j0 = (w.tile_lo + t) * M_KEYS;
       const bool plain = j0 + M_KEYS <= x.start && (a.window <= 0 || j0 >= x.kv_len - a.window);
+      Sight<(WK + 31) / 32> sight[2];
+      if (!plain && live) {
+        sight[0].words(a, token[0], j0 + key0, x.start);
+        sight[1].words(a, token[1], j0 + key0, x.start);
+      }
       bf16* kt = kv_sh + (t % STAGES) * 2 * tile_elems;
       bf16* vt = kt + tile_elems;
       if (!plain) {
@@ -162,20 +167,16 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
             mx[i >> 1] = fmaxf(mx[i >> 1], s[nt][i]);
           }
       } else {
-        uint64_t bits[2];
+        constexpr int NW = (WK + 31) / 32;
+        uint32_t bits[2][NW];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int* row_mask = a.mask + (size_t)token[i] * a.words;
-          bits[i] = 0;
-#pragma unroll
-          for (int h = 0; h < WK; h += 32) bits[i] |= (uint64_t)seen_bits(a, row_mask, j0 + key0 + h, x.start, x.kv_len, lo[i]) << h;
-        }
+        for (int i = 0; i < 2; ++i) sight[i].bits(bits[i], j0 + key0, x.start, x.kv_len, lo[i]);
 #pragma unroll
         for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int k = nt * 8 + (lane & 3) * 2 + (i & 1);
-            s[nt][i] = (bits[i >> 1] >> k) & 1 ? s[nt][i] * a.scale_log2 : -CUDART_INF_F;
+            s[nt][i] = (bits[i >> 1][(nt * 8) / 32] >> (k & 31)) & 1 ? s[nt][i] * a.scale_log2 : -CUDART_INF_F;
             mx[i >> 1] = fmaxf(mx[i >> 1], s[nt][i]);
           }
       }
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
     }
     __syncthreads();                                             // the tiles' memory is free
     const bool loose = loose_sh != 0, whole = w.begins && w.ends;
-    const size_t slab = slab_of(blockIdx.x, w.begins) * ROWS;
+    const size_t slab = slab_of(blockIdx.x, w.begins);
     // two neighbouring numbers of a row, sums with reference mr and total lr
     auto put = [&](int row, int d, float v0, float v1, float inv) {
       if (loose) {
@@ -243,7 +244,9 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
         bf16* dst = (bf16*)a.out + ((size_t)(x.q0 + r / g) * a.nq + w.kvh * g + r % g) * hd + d;
         *reinterpret_cast<uint32_t*>(dst) = pack_bf16(v0 * inv, v1 * inv);
       } else {
-        *reinterpret_cast<float2*>(a.part_o + (slab + row) * hd + d) = make_float2(v0, v1);
+        float* dst = a.part_o + (slab * hd + d) * ROWS + row;
+        dst[0] = v0;
+        dst[ROWS] = v1;
       }
     };
     if constexpr (KEY_WARPS == 1) {
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
         const int row = ra + 8 * i;
         if (row >= rows) continue;
         const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
-        if (!whole && (lane & 3) == 0) *reinterpret_cast<float2*>(a.part_ml + (slab + row) * 2) = make_float2(m[i], l[i]);
+        if (!whole && (lane & 3) == 0) *reinterpret_cast<float2*>(a.part_ml + (slab * ROWS + row) * 2) = make_float2(m[i], l[i]);
 #pragma unroll
         for (int dn = 0; dn < NO; ++dn)
           if (dn * 8 < hd) put(row, dn * 8 + (lane & 3) * 2, o[dn][2 * i], o[dn][2 * i + 1], inv);
@@ -271,8 +274,9 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
       }
       __syncthreads();
       const int pairs = hd >> 1;
-      for (int i = tid; i < rows * pairs; i += M_THREADS) {
-        const int row = i / pairs, d = (i - row * pairs) * 2;
+      for (int i = tid; i < ROWS * pairs; i += M_THREADS) {
+        const int row = whole ? i / pairs : i % ROWS, d = (whole ? i - row * pairs : i / ROWS) * 2;      // (as they are stored side by side)
+        if (row >= rows) continue;
         const int first = (row >> 4) * KEY_WARPS * 16 + (row & 15);      // the row in its first warp's share
         float M = -CUDART_INF_F, L = 0.f, v0 = 0.f, v1 = 0.f;
 #pragma unroll
@@ -287,7 +291,7 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
           v0 += f * v.x;
           v1 += f * v.y;
         }
-        if (!whole && d == 0) *reinterpret_cast<float2*>(a.part_ml + (slab + row) * 2) = make_float2(M, L);
+        if (!whole && d == 0) *reinterpret_cast<float2*>(a.part_ml + (slab * ROWS + row) * 2) = make_float2(M, L);
         put(row, d, v0, v1, L == 0.f ? 0.f : 1.f / L);
       }
     }
@@ -301,7 +305,7 @@ static int key_warps(int max_rows) { return max_rows <= 16 ? 4 : max_rows <= 32 
 static int blocks_per_sm(int hd) { return hd <= 64 ? 3 : hd <= 128 ? 2 : 1; }
 
 bool mma_takes(int hd) { return hd % 16 == 0 && hd <= 256; }
-Form mma_form(int hd, int max_rows, int sms) { return Form{blocks_per_sm(hd) * sms, 64 / key_warps(max_rows)}; }
+Form mma_form(int hd, int max_rows, int sms) { return Form{blocks_per_sm(hd) * sms, 64 / key_warps(max_rows), M_KEYS}; }
 
 template <int HD_MAX, int KEY_WARPS, int STAGES>
 static int run_form(const Args& a, int max_rows, int sms, cudaStream_t stream) {
@@ -310,7 +314,7 @@ static int run_form(const Args& a, int max_rows, int sms, cudaStream_t stream) {
   const cudaError_t e = cudaFuncSetAttribute(tree_mma_kernel<HD_MAX, KEY_WARPS, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", smem);
   launch_pdl(tree_mma_kernel<HD_MAX, KEY_WARPS, STAGES>, dim3(blocks), dim3(M_THREADS), smem, stream, a);
-  launch_pdl(tree_merge_kernel<bf16, F::ROWS, M_KEYS>, dim3(blocks, (min(max_rows, F::ROWS) + 7) / 8), dim3(256), 0, stream, a, blocks);
+  launch_merge<bf16, F::ROWS, M_KEYS>(a, blocks, max_rows, stream);
   return launched();
 }
 // Stages: as many as leave room for another block on the SM.

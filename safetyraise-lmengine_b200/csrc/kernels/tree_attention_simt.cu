@@ -114,7 +114,11 @@ __global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const __grid_const
             bool sees = true;
             if (!plain) {
               const int t = x.q0 + (r0 + warp * S_OWN + o) / g;
-              sees = (seen_bits(a, a.mask + (size_t)t * a.words, j0, x.start, x.kv_len, first_key_of(a, t, x.start)) >> lane) & 1;
+              Sight<1> sight;
+              uint32_t bits[1];
+              sight.words(a, t, j0, x.start);
+              sight.bits(bits, j0, x.start, x.kv_len, first_key_of(a, t, x.start));
+              sees = (bits[0] >> lane) & 1;
             }
             const float v = sees ? s[o] * a.scale_log2 : -CUDART_INF_F;
             const float m_new = fmaxf(m[o], warp_max(v));
@@ -157,7 +161,7 @@ __global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const __grid_const
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     const bool whole = w.begins && w.ends;
-    const size_t slab = slab_of(blockIdx.x, w.begins) * S_ROWS;
+    const size_t slab = slab_of(blockIdx.x, w.begins);
 #pragma unroll
     for (int o = 0; o < S_OWN; ++o) {
       if (o >= own) continue;
@@ -169,16 +173,16 @@ __global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const __grid_const
         for (int i = 0; i < DIMS; ++i)
           if (lane + 32 * i < a.hd) dst[lane + 32 * i] = from_float<T>(acc[o][i] * inv);
       } else {
-        if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + (slab + row) * 2) = make_float2(m[o], l[o]);
+        if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + (slab * S_ROWS + row) * 2) = make_float2(m[o], l[o]);
 #pragma unroll
         for (int i = 0; i < DIMS; ++i)
-          if (lane + 32 * i < a.hd) a.part_o[(slab + row) * a.hd + lane + 32 * i] = acc[o][i];
+          if (lane + 32 * i < a.hd) a.part_o[(slab * a.hd + lane + 32 * i) * S_ROWS + row] = acc[o][i];
       }
     }
   }
 }
 
-Form simt_form(int hd, int sms) { return Form{(hd <= 64 ? 4 : hd <= 128 ? 2 : 1) * sms, S_ROWS}; }
+Form simt_form(int hd, int sms) { return Form{(hd <= 64 ? 4 : hd <= 128 ? 2 : 1) * sms, S_ROWS, S_KEYS}; }
 
 template <typename T, int DIMS, bool COPY>
 static int run_form(const Args& a, int max_rows, int sms, cudaStream_t stream) {
@@ -186,7 +190,7 @@ static int run_form(const Args& a, int max_rows, int sms, cudaStream_t stream) {
   const cudaError_t e = cudaFuncSetAttribute(tree_simt_kernel<T, DIMS, COPY>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", smem);
   launch_pdl(tree_simt_kernel<T, DIMS, COPY>, dim3(blocks), dim3(S_THREADS), smem, stream, a);
-  launch_pdl(tree_merge_kernel<T, S_ROWS, S_KEYS>, dim3(blocks, (min(max_rows, S_ROWS) + 7) / 8), dim3(256), 0, stream, a, blocks);
+  launch_merge<T, S_ROWS, S_KEYS>(a, blocks, max_rows, stream);
   return launched();
 }
 template <typename T, bool COPY>

@@ -9,7 +9,8 @@
 // warps form the weights of a tile, the tensor core works for the other, and three stages of keys and values (six of heads of
 // 64) are in flight.  At the end of a piece the two streams' sums are joined as they are read from tensor memory (a warp reads
 // the same lanes of both; each stream's warps write half of the columns).
-// Warp 0 fetches (a lane a page box), one thread of warp 1 issues the MMAs, warps 2-5 and 6-9 are the streams' softmax.  A block
+// Warps 0 and 10 fetch keys and values (a lane a page box), one thread of warp 1 issues the MMAs, warps 2-5 and 6-9 are the
+// streams' softmax.  A block
 // stays for all of its pieces: the fetches run ahead across them, and the block count is the SMs'.
 //
 // A weight is rounded to bfloat16 for the product with the values.  O is rescaled only when a row's maximum has grown by more
@@ -23,7 +24,7 @@ namespace tree {
 
 using namespace fmha;
 
-constexpr int T_ROWS = 128, T_KEYS = 128, T_THREADS = 320, T_SOFTMAX = 256;
+constexpr int T_ROWS = 128, T_KEYS = 128, T_THREADS = 352, T_SOFTMAX = 256;
 constexpr float T_RESCALE_ABOVE = 8.f;             // log2 of the growth of a row's maximum that O is rescaled for
 
 template <int HD>
@@ -33,39 +34,16 @@ struct TmaForm {
   static constexpr int SMEM = TILE * (1 + 2 * STAGES) + 1024 + (4 * STAGES + 7) * 8;
 };
 
-// The row's maximum over the keys that it sees (bits), and its weights exp2(S * scale - base) as bfloat16 pairs over the first 64
-// columns of S; the sum of the weights.
-__device__ __forceinline__ float row_max_seen(const Row& r, const uint32_t (&bits)[4]) {
-  float m[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-  auto part = [&](const uint32_t (&v)[32], uint32_t b) {
+// Scores of keys that the row does not see become -inf (the score scale is positive): a weight of zero.
+__device__ __forceinline__ void mask_row(Row& r, const uint32_t (&bits)[4]) {
+  auto part = [&](uint32_t (&v)[32], uint32_t b) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) m[j & 3] = fmaxf(m[j & 3], (b >> j) & 1 ? __uint_as_float(v[j]) : -CUDART_INF_F);
+    for (int j = 0; j < 32; ++j) v[j] = (b >> j) & 1 ? v[j] : 0xff800000u;
   };
   part(r.a, bits[0]);
   part(r.b, bits[1]);
   part(r.c, bits[2]);
   part(r.d, bits[3]);
-  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-}
-__device__ __forceinline__ float row_exp_seen(uint32_t s_addr, const Row& r, float scale, float base, const uint32_t (&bits)[4]) {
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  auto part = [&](const uint32_t (&v)[32], uint32_t b, int c) {
-    uint32_t pk[16];
-#pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-      const float p0 = (b >> j) & 1 ? ex2(fmaf(__uint_as_float(v[j]), scale, -base)) : 0.f;
-      const float p1 = (b >> (j + 1)) & 1 ? ex2(fmaf(__uint_as_float(v[j + 1]), scale, -base)) : 0.f;
-      pk[j >> 1] = pack2(p0, p1);
-      sum[j & 2] += p0;
-      sum[(j & 2) + 1] += p1;
-    }
-    tmem_st16(s_addr + (c >> 1), pk);
-  };
-  part(r.a, bits[0], 0);
-  part(r.b, bits[1], 32);
-  part(r.c, bits[2], 64);
-  part(r.d, bits[3], 96);
-  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 template <int HD>
@@ -86,7 +64,9 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   uint64_t* p_ready = s_full + 2;                  // [2]
   uint64_t* o_done = p_ready + 2;                  // [2]
   uint64_t* q_full = o_done + 2;
-  __shared__ Walk<T_ROWS, T_KEYS> walk_sh[3];
+  __shared__ Walk<T_ROWS, T_KEYS> walk_sh;
+  __shared__ Piece piece_sh;
+  __shared__ int more_sh;
   __shared__ uint32_t tmem_sh;
   __shared__ int loose_sh, failed_sh;
 
@@ -121,80 +101,55 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   pdl_trigger();
 
   const int g = a.nq / a.nkv;
-  // the walk lies in shared memory between pieces, one for each role: its numbers would cost the softmax registers
   using Walks = Walk<T_ROWS, T_KEYS>;
-  const int role = min(warp, 2);
-  Piece w;
-  {
-    Walks walk;
+  Walks walk;
+  if (warp <= 2 || warp == 10) {
     walk.init(a, blockIdx.x, gridDim.x, blockIdx.x == 0 && warp == 0);
-    if ((warp <= 2) && lane == 0) walk_sh[role] = walk;
+    if (warp == 2 && lane == 0) walk_sh = walk;    // (the softmax warps keep theirs in shared memory: its numbers would cost them registers)
   }
-  __syncthreads();
-  // read: by every warp of the role; kept: by one of them once all have read (the softmax warps meet between two pieces)
-  auto next = [&] {
-    Walks walk = walk_sh[role];
-    const bool more = walk.next(a, w);
-    if (role < 2) {
-      __syncwarp();
-      if (lane == 0) walk_sh[role] = walk;
-      __syncwarp();
-    } else {
-      asm volatile("bar.sync 1, %0;" ::"n"(T_SOFTMAX) : "memory");
-      if (threadIdx.x == 64) walk_sh[2] = walk;
-    }
-    return more;
-  };
-  auto first_key = [&] { return a.window > 0 ? max(0, w.x.start - a.window + 1) : 0; };
 
-  if (warp == 0) {
-    // ---------------- TMA producer ----------------
+  if (warp == 0 || warp == 10) {
+    // ---------------- TMA producers: keys, values ----------------
+    const bool keys = warp == 0;
+    const CUtensorMap* map = keys ? &map_k : &map_v;
+    uint8_t* ring = keys ? k_t : v_t;
+    uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
     const int ps = a.page_size, box_rows = ps < T_KEYS ? ps : T_KEYS, boxes = T_KEYS / box_rows;
     int k = 0;                                     // tiles so far
     bool ok = true;
-    int k_loads = 0, v_loads = 0;
-    while (ok && next()) {
+    Piece w;
+    while (ok && walk.next(a, w)) {
       const int* table = a.block_table + (size_t)w.e * a.table_stride;
-      const int first = first_key();
-      for (int t = w.tile_lo; t < w.tile_hi && ok; ++t, ++k) {
+      const int first = a.window > 0 ? max(0, w.x.start - a.window + 1) : 0;
+      // the lane's page of a tile, looked up a tile ahead (behind the entry's last key: page 0, which nobody sees)
+      auto page_of = [&](int t) {
+        const int key = t * T_KEYS + lane * box_rows;
+        return lane < boxes && t < w.tile_hi && key < w.x.kv_len ? table[key / ps] : 0;
+      };
+      int page_next = page_of(w.tile_lo);
+      for (int t = w.tile_lo; t < w.tile_hi; ++t, ++k) {
         const int s = k % STAGES;
-        const uint32_t parity = ((k / STAGES) & 1) ^ 1;
-        int row = 0;
-        if (lane < boxes) {                        // the lanes' lookups of a tile overlap
-          const int key = t * T_KEYS + lane * box_rows, pg = key / ps;
-          int page = 0;
-          if (key < w.x.kv_len) {
-            page = table[pg];
-            if (page < 0 || page >= a.num_pages) {
-              if (key + box_rows > first) atomicExch(a.err_flag, ERR_PAGE);      // (pages behind a window are given back)
-              page = 0;
-            }
-          }
-          row = (page * a.nkv + w.kvh) * ps + (key - pg * ps);
+        int page = page_next;
+        page_next = page_of(t + 1);
+        const int key = t * T_KEYS + lane * box_rows;
+        if (page < 0 || page >= a.num_pages) {
+          if (key + box_rows > first) atomicExch(a.err_flag, ERR_PAGE);      // (pages behind a window are given back)
+          page = 0;
         }
-        auto load = [&](const CUtensorMap* map, uint8_t* tile, uint64_t* full) {
-          if (lane == 0) mbar_expect_tx(full, TILE);
-          __syncwarp();
-          if (lane < boxes) {
+        const int row = (page * a.nkv + w.kvh) * ps + key % ps;
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((k / STAGES) & 1) ^ 1, a.err_flag, 81));
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(&full[s], TILE);
+        __syncwarp();
+        uint8_t* tile = ring + s * TILE + lane * box_rows * 128;
+        if (lane < boxes) {
 #pragma unroll
-            for (int c = 0; c < HD; c += 64) tma_load_2d(tile + c * (T_KEYS * 2) + lane * box_rows * 128, map, full, c, row);
-          }
-        };
-        ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[s], parity, a.err_flag, 81));
-        if (!ok) break;
-        load(&map_k, k_t + s * TILE, &k_full[s]);
-        ++k_loads;
-        ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[s], parity, a.err_flag, 82));
-        if (!ok) break;
-        load(&map_v, v_t + s * TILE, &v_full[s]);
-        ++v_loads;
+          for (int c = 0; c < HD; c += 64) tma_load_2d(tile + c * (T_KEYS * 2), map, &full[s], c, row);
+        }
       }
     }
     if (!ok)                                       // copies in flight end before the block does
-      for (int back = 1; back <= STAGES; ++back) {
-        if (back <= k_loads) mbar_wait(&k_full[(k_loads - back) % STAGES], ((k_loads - back) / STAGES) & 1, a.err_flag, 81);
-        if (back <= v_loads) mbar_wait(&v_full[(v_loads - back) % STAGES], ((v_loads - back) / STAGES) & 1, a.err_flag, 82);
-      }
+      for (int back = 1; back <= STAGES && back <= k; ++back) mbar_wait(&full[(k - back) % STAGES], ((k - back) / STAGES) & 1, a.err_flag, 82);
     __syncwarp();
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
@@ -205,7 +160,8 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     int k = 0, piece = 0;
     uint32_t done[2] = {0, 0};                     // tiles of either stream so far
     bool ok = true;
-    while (next()) {                            // (the whole warp walks, one lane issues)
+    Piece w;
+    while (walk.next(a, w)) {                      // (the whole warp walks, one lane issues)
       if (lane == 0 && ok) {
         const int tiles = w.tile_hi - w.tile_lo;
         auto issue_s = [&](int t) {                // S_i = Q . K_t^T
@@ -255,10 +211,13 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     uint32_t done = 0;                             // tiles of this stream so far
     int k = 0;                                     // tiles of the block so far
     bool ok = true;
-    while (next()) {
-      const Entry& x = w.x;
+    const Piece& w = piece_sh;
+    const Entry& x = w.x;
+    for (;;) {
+      if (threadIdx.x == 64) more_sh = walk_sh.next(a, piece_sh);      // (the last piece's readers have met)
+      meet();
+      if (!more_sh) break;
       const int rows_total = x.q_len * g, r0 = w.block * T_ROWS, rows = min(T_ROWS, rows_total - r0), tiles = w.tile_hi - w.tile_lo;
-      const int first = first_key();
       // the rows -> shared memory, swizzled (zeros behind the last), eight loads of a thread in flight; the products that read the last
       // piece's are done (their tiles were waited for)
       const bf16* q = (const bf16*)a.q;
@@ -285,39 +244,38 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       if (lane == 0) mbar_arrive(q_full);
 
       const int r = min(r0 + row, rows_total - 1), token = x.q0 + r / g;
-      const int lo = first_key_of(a, token, x.start);
-      const int* row_mask = a.mask + (size_t)token * a.words;
       const bool live = ew * 32 < rows;            // some row of the warp is one
       float m_run = -CUDART_INF_F, l_run = 0.f;
       bool any = false;
       for (int t = i; t < tiles && ok; t += 2, ++done, any = true) {
         const int j0 = (w.tile_lo + t) * T_KEYS;
+        // every row sees every key of a tile between the window's last edge and the drafted tokens
+        const bool plain = j0 + T_KEYS <= x.start && (a.window <= 0 || j0 >= x.kv_len - a.window);
+        uint32_t bits[4];
+        if (!plain && live) {
+          Sight<4> sight;
+          sight.words(a, token, j0, x.start);
+          sight.bits(bits, j0, x.start, x.kv_len, first_key_of(a, token, x.start));
+        }
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[i], done & 1, a.err_flag, 87));
         if (!ok) break;
         fence_after();
-        // every row sees every key of a tile between the window's last edge and the drafted tokens
-        const bool plain = j0 + T_KEYS <= x.start && (a.window <= 0 || j0 >= x.kv_len - a.window);
         if (!plain) {
           // values of no key of the entry become zeros, and those that are no numbers are taken out
           const int s = (k + t) % STAGES;
           ok = __all_sync(0xffffffffu, mbar_wait(&v_full[s], ((k + t) / STAGES) & 1, a.err_flag, 88));
           if (!ok) break;
-          const uint32_t vt = s32(v_t + s * TILE);
+          uint8_t* vt = v_t + s * TILE;
+          const int first = a.window > 0 ? max(0, x.start - a.window + 1) - j0 : 0, behind = x.kv_len - j0;
           bool loose = false;
-          for (int idx = ew * 32 + lane; idx < T_KEYS * CHUNKS; idx += 128) {
-            const int key = idx / CHUNKS;
-            const uint32_t at = tile_addr(vt, key, idx % CHUNKS);
-            uint4 v;
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-            bool change;
-            if (j0 + key < first || j0 + key >= x.kv_len) {
-              v = make_uint4(0, 0, 0, 0);
-              change = true;
-            } else {
-              change = take_loose(v);
-              loose |= change;
-            }
-            if (change) asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+#pragma unroll 4
+          for (int n = 0; n < T_KEYS * CHUNKS / 128; ++n) {
+            const int idx = n * 128 + row, key = idx / CHUNKS;
+            uint4* at = reinterpret_cast<uint4*>(vt + tile_addr(0, key, idx % CHUNKS));
+            uint4 v = *at;
+            const bool there = key >= first && key < behind, change = take_loose(v);
+            loose |= there && change;
+            if (!there || change) *at = there ? v : make_uint4(0, 0, 0, 0);
           }
           if (loose) loose_sh = 1;
           fence_async_smem();
@@ -325,11 +283,8 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (live) {
           Row srow;
           load_row(s_addr, srow);
-          uint32_t bits[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-          if (!plain)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) bits[c] = seen_bits(a, row_mask, j0 + 32 * c, x.start, x.kv_len, lo);
-          const float mx = (plain ? row_max<false>(srow, 0, T_KEYS) : row_max_seen(srow, bits)) * a.scale_log2;
+          if (!plain) mask_row(srow, bits);
+          const float mx = row_max<false>(srow, 0, T_KEYS) * a.scale_log2;
           const bool grow = mx > m_run + T_RESCALE_ABOVE || m_run == -CUDART_INF_F;
           const float m_new = grow ? fmaxf(mx, m_run) : m_run;
           if (any && __any_sync(0xffffffffu, m_new != m_run)) {
@@ -349,7 +304,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           }
           m_run = m_new;
           const float base = m_run == -CUDART_INF_F ? 0.f : m_run;
-          l_run += plain ? row_exp<false>(s_addr, srow, a.scale_log2, base, 0, T_KEYS) : row_exp_seen(s_addr, srow, a.scale_log2, base, bits);
+          l_run += row_exp<false>(s_addr, srow, a.scale_log2, base, 0, T_KEYS);
           tmem_wait_st();
         }
         fence_before();
@@ -388,8 +343,8 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const float L = two ? f0 * s0.y + f1 * s1.y : f0 * s0.y;
         const bool mine = row < rows, whole = w.begins && w.ends;
         const float inv = L == 0.f ? 0.f : 1.f / L;
-        const size_t slab = slab_of(blockIdx.x, w.begins) * T_ROWS + row;
-        if (!whole && mine && i == 0) *reinterpret_cast<float2*>(a.part_ml + slab * 2) = make_float2(M, L);
+        const size_t slab = slab_of(blockIdx.x, w.begins);
+        if (!whole && mine && i == 0) *reinterpret_cast<float2*>(a.part_ml + (slab * T_ROWS + row) * 2) = make_float2(M, L);
         bf16* dst = (bf16*)a.out + ((size_t)token * a.nq + w.kvh * g + r % g) * HD;
         const uint32_t both = tmem + 256 + lane_addr;
 #pragma unroll 1
@@ -419,8 +374,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                              pack2(o[8 * n + 4] * inv, o[8 * n + 5] * inv), pack2(o[8 * n + 6] * inv, o[8 * n + 7] * inv));
           } else if (mine) {
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
-              *reinterpret_cast<float4*>(a.part_o + slab * HD + c + 4 * n) = make_float4(o[4 * n], o[4 * n + 1], o[4 * n + 2], o[4 * n + 3]);
+            for (int n = 0; n < 16; ++n) a.part_o[(slab * HD + c + n) * T_ROWS + row] = o[n];
           }
         }
         fence_before();
@@ -451,7 +405,7 @@ bool tcgen05_takes(int hd, int page_size) {
   return (hd == 64 || hd == 128) && (page_size == 8 || page_size == 16 || page_size == 32 || page_size == 64 ||
                                      (page_size > 0 && page_size % T_KEYS == 0));
 }
-Form tcgen05_form(int sms) { return Form{sms, T_ROWS}; }
+Form tcgen05_form(int sms) { return Form{sms, T_ROWS, T_KEYS}; }
 
 template <int HD>
 static int run_form(const Args& a, int max_rows, int sms, cudaStream_t stream) {
@@ -463,7 +417,7 @@ static int run_form(const Args& a, int max_rows, int sms, cudaStream_t stream) {
   const cudaError_t e = cudaFuncSetAttribute(tree_tcgen05_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, TmaForm<HD>::SMEM);
   if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", TmaForm<HD>::SMEM);
   launch_pdl(tree_tcgen05_kernel<HD>, dim3(sms), dim3(T_THREADS), TmaForm<HD>::SMEM, stream, mk, mv, a);
-  launch_pdl(tree_merge_kernel<bf16, T_ROWS, T_KEYS>, dim3(sms, (min(max_rows, T_ROWS) + 7) / 8), dim3(256), 0, stream, a, sms);
+  launch_merge<bf16, T_ROWS, T_KEYS>(a, sms, max_rows, stream);
   return launched();
 }
 int run_tcgen05(const Args& a, int max_rows, int sms, cudaStream_t stream) {
