@@ -16,7 +16,7 @@ static tree::Form form_of(Kind kind, int hd, int max_rows, int sms) {
 
 // float32 words of workspace that srlm_tree_attention wants for these sizes, or -1 where it refuses them.
 extern "C" long long srlm_tree_attention_workspace(int dtype, int nq, int nkv, int hd, int page_size, int max_q_len, int sms) {
-  if ((dtype != DT_F32 && dtype != DT_BF16) || nq <= 0 || nkv <= 0 || nq % nkv || hd <= 0 || hd > 256 || page_size <= 0 ||
+  if ((dtype != DT_F32 && dtype != DT_BF16) || nq <= 0 || nkv <= 0 || nkv > 65535 || nq % nkv || hd <= 0 || hd > 256 || page_size <= 0 ||
       max_q_len <= 0 || sms <= 0 || (long long)max_q_len * (nq / nkv) > (1 << 24)) {
     refuse(ST_BAD_SIZE, "tree_attention: dtype=%d nq=%d nkv=%d hd=%d page_size=%d max_q_len=%d (needs nq %% nkv == 0, hd <= 256)",
            dtype, nq, nkv, hd, page_size, max_q_len);
@@ -24,7 +24,7 @@ extern "C" long long srlm_tree_attention_workspace(int dtype, int nq, int nkv, i
   }
   const int max_rows = max_q_len * (nq / nkv);
   const tree::Form f = form_of(kind_of(dtype, hd, page_size, max_rows), hd, max_rows, sms);
-  return 2ll * f.blocks * f.rows * (hd + 2);
+  return 2ll * f.blocks * f.rows * (hd + 2) + 4ll * f.blocks;
 }
 
 // q, out [T, nq, hd]; caches [num_pages, nkv, page_size, hd]; block_table [n, table_stride]; cu_q [n + 1]; kv_lens [n]; mask
@@ -47,9 +47,10 @@ extern "C" int srlm_tree_attention(const void* q, const void* k_cache, const voi
   if (units * tiles > 2147483647.0)
     return refuse(ST_BAD_SIZE, "tree_attention: %d entries of up to %d tokens and %d pages are more work than a call takes", n, max_q_len,
                   table_stride);
+  float* ml = work + 2ll * f.blocks * f.rows * hd;      // (sizes are multiples of 16 bytes)
   tree::Args a{q, k_cache, v_cache, out, block_table, table_stride, cu_q, kv_lens, mask, words, std::min(max_q_len, 32 * words), positions, n, T,
                nq, nkv, hd, page_size, (int)num_pages, scale * 1.4426950408889634f, window, 1, err_flag, work,
-               work + 2ll * f.blocks * f.rows * hd};
+               ml, reinterpret_cast<int4*>(ml + 4ll * f.blocks * f.rows)};
   if (kind != SIMT) {
     if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) % 16)
       return refuse(ST_BAD_ALIGN, "tree_attention: bfloat16 tensors start on 16-byte boundaries");

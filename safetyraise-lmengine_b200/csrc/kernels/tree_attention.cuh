@@ -19,6 +19,8 @@
 
 #include <math_constants.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace srlm {
@@ -48,6 +50,8 @@ struct Args {
   int* err_flag;
   float* part_o;             // slabs [2 C][hd][ROWS]: neighbouring rows side by side, as the threads that write and read them are
   float* part_ml;            // [2 C][ROWS][2]: reference maximum (log2 units), sum of weights
+  int4* part_units;          // [C]: the unit that begins in share C and goes on behind it: slabs (0: none such), first row of its
+                             // entry's rows, first token of the entry, KV head | rows << 16
 };
 
 struct Entry {
@@ -104,9 +108,7 @@ struct Walk {
     return pos < longer ? pos / (each + 1) : more + (pos - longer) / each;
   }
 
-  // All lanes of a warp.  share: which of `blocks_there`; the entries' tiles are counted by the warp, 32 entries a turn.  LAST: stands
-  // at the share's last tile instead of its first.
-  template <bool LAST = false>
+  // All lanes of a warp.  share: which of `blocks_there`; the entries' tiles are counted by the warp, 32 entries a turn.
   __device__ __forceinline__ void init(const Args& a, int share, int blocks_there, bool flag) {
     const int lane = threadIdx.x & 31;
     int w = 0, total = 0;
@@ -122,7 +124,6 @@ struct Walk {
     at = first_of(share);
     end = first_of(share + 1);
     // the entry that holds the tile
-    const int pos = LAST ? end - 1 : at;
     int before = 0;
     for (int e0 = 0; e0 < a.n; e0 += 32) {
       if (a.n > 32) w = e0 + lane < a.n ? weight(a, entry_of<ROWS, KEYS>(a, e0 + lane)) : 0;
@@ -132,7 +133,7 @@ struct Walk {
         const int v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
       }
-      const unsigned beyond = __ballot_sync(0xffffffffu, before + upto > pos);
+      const unsigned beyond = __ballot_sync(0xffffffffu, before + upto > at);
       if (beyond) {
         const int l = __ffs(beyond) - 1;
         e = e0 + l;
@@ -250,72 +251,102 @@ __device__ __noinline__ float loose_values(const Args& a, int start, int kv_len,
   return sum;
 }
 
-// Adds the slabs of the unit that begins in share blockIdx.x and goes on behind it: out = sum_z O_z 2^(m_z - M) / sum_z l_z
-// 2^(m_z - M), M the largest reference of a slab that saw a key.  A lane has a row and MERGE_DIMS of its dimensions (a warp of fewer
-// rows than lanes several such runs); blockIdx.y and z run over groups of MERGE_WARPS runs and 32 rows.  The division of the work is
-// found while the kernel ahead still runs (its own blocks have waited for all that it reads of the lengths).
-constexpr int MERGE_WARPS = 4, MERGE_DIMS = 8;
+// What a block leaves for the merge beside its slabs, by one thread: the unit that goes on behind its share (it begins in the last
+// piece), or that there is none.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ void leave_unit(const Args& a, const Walk<ROWS, KEYS>& w, const Piece& p) {
+  if (!p.begins || p.ends) return;
+  const int to = w.at + (p.x.first_tile + p.x.tiles - p.tile_hi), r0 = p.block * ROWS;
+  a.part_units[blockIdx.x] = make_int4(w.share_of(to - 1) - blockIdx.x + 1, r0, p.x.q0,
+                                       p.kvh | min(ROWS, p.x.q_len * (a.nq / a.nkv) - r0) << 16);
+}
 
-template <typename T, int ROWS, int KEYS>
-__global__ void __launch_bounds__(32 * MERGE_WARPS) tree_merge_kernel(const __grid_constant__ Args a, int blocks_there) {
+// Adds the slabs of the unit that begins in share blockIdx.x and goes on behind it: out = sum_z O_z 2^(m_z - M) / sum_z l_z
+// 2^(m_z - M), M the largest reference of a slab that saw a key.  A lane has a row and MERGE_DIMS of its dimensions (of units of
+// fewer rows than lanes, a warp has several such runs); the block's warps take the slabs in turn and add up their shares in shared
+// memory, so that a row of many slabs costs a few reads one behind another.
+constexpr int MERGE_WARPS = 8, MERGE_DIMS = 16;
+
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(32 * MERGE_WARPS) tree_merge_kernel(const __grid_constant__ Args a) {
   constexpr int RL = ROWS < 32 ? ROWS : 32, RUNS = 32 / RL;            // rows, runs of a warp
+  __shared__ float acc_sh[MERGE_WARPS][MERGE_DIMS][32];
+  __shared__ float2 ml_sh[MERGE_WARPS][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int share = blockIdx.x, row = blockIdx.z * RL + lane % RL;
-  const int d0 = ((blockIdx.y * MERGE_WARPS + warp) * RUNS + lane / RL) * MERGE_DIMS;
-  Walk<ROWS, KEYS> w;
-  w.template init<true>(a, share, blocks_there, false);
-  bool mine = w.at < w.end;
-  int share_last = 0;
-  T* dst = nullptr;
-  if (mine) {
-    const int unit = (w.end - 1 - w.base) / w.x.tiles, from = w.base + unit * w.x.tiles, to = from + w.x.tiles;
-    const int kvh = unit / w.x.blocks, g = a.nq / a.nkv, r = (unit - kvh * w.x.blocks) * ROWS + row;
-    // else another share's unit, or a whole one, or no row
-    mine = from >= w.at && to > w.end && row < ROWS && r < w.x.q_len * g && d0 < a.hd;
-    if (mine) {
-      share_last = w.share_of(to - 1);
-      dst = (T*)a.out + ((size_t)(w.x.q0 + r / g) * a.nq + kvh * g + r % g) * a.hd + d0;
-    }
-  }
+  const int share = blockIdx.x, row = blockIdx.z * RL + lane % RL, d0 = (blockIdx.y * RUNS + lane / RL) * MERGE_DIMS;
   pdl_wait();
   pdl_trigger();
-  if (!mine) return;
-  const int slabs = share_last - share + 1;
-  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row;
-  auto slab = [&](int z) { return slab_of(share + z, z == 0); };
-  float M = -CUDART_INF_F;
-#pragma unroll 4
-  for (int z = 0; z < slabs; ++z) {
-    const float2 v = ml[slab(z) * ROWS];
-    if (v.y > 0.f) M = fmaxf(M, v.x);
-  }
-  float acc[MERGE_DIMS], L = 0.f;
+  const int4 unit = a.part_units[share];
+  const int slabs = unit.x, kvh = unit.w & 0xffff, rows = unit.w >> 16;
+  if (slabs == 0 || blockIdx.z * RL >= rows) return;
+  const int dims = min(MERGE_DIMS, a.hd - d0);
+  const bool there = row < rows && dims > 0;
+  float acc[MERGE_DIMS], M = -CUDART_INF_F, L = 0.f;
 #pragma unroll
   for (int i = 0; i < MERGE_DIMS; ++i) acc[i] = 0.f;
-  const int dims = min(MERGE_DIMS, a.hd - d0);
-#pragma unroll 2
-  for (int z = 0; z < slabs; ++z) {
-    const float2 v = ml[slab(z) * ROWS];
-    const float* src = a.part_o + (slab(z) * a.hd + d0) * ROWS + row;
-    float o[MERGE_DIMS];
+  if (there)
+    for (int z = warp; z < slabs; z += MERGE_WARPS) {
+      const size_t slab = slab_of(share + z, z == 0);
+      const float2 v = *reinterpret_cast<const float2*>(a.part_ml + (slab * ROWS + row) * 2);
+      const float* src = a.part_o + (slab * a.hd + d0) * ROWS + row;
+      float o[MERGE_DIMS];
 #pragma unroll
-    for (int i = 0; i < MERGE_DIMS; ++i) o[i] = i < dims ? src[i * ROWS] : 0.f;
-    const float f = v.y > 0.f ? exp2f(v.x - M) : 0.f;
-    L += v.y != v.y ? v.y : f * v.y;                                   // (a score that was no number makes the row none)
-    if (f > 0.f)                                                       // (a slab of no key holds nothing)
+      for (int i = 0; i < MERGE_DIMS; ++i) o[i] = i < dims ? src[i * ROWS] : 0.f;
+      if (v.y > 0.f) {                                                 // (a slab of no key holds nothing)
+        const float m_new = fmaxf(M, v.x), f = exp2f(v.x - m_new), old = exp2f(M - m_new);
+        M = m_new;
+        L = L * old + f * v.y;
 #pragma unroll
-      for (int i = 0; i < MERGE_DIMS; ++i) acc[i] += f * o[i];
+        for (int i = 0; i < MERGE_DIMS; ++i) acc[i] = acc[i] * old + f * o[i];
+      } else if (v.y != v.y) {
+        L = v.y;                                                       // (a score that was no number makes the row none)
+      }
+    }
+  ml_sh[warp][lane] = make_float2(M, L);
+#pragma unroll
+  for (int i = 0; i < MERGE_DIMS; ++i) acc_sh[warp][i][lane] = acc[i];
+  __syncthreads();
+  if (!there) return;
+  // each warp writes its part of the dimensions
+  float f[MERGE_WARPS], top = -CUDART_INF_F, sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < MERGE_WARPS; ++k) top = fmaxf(top, ml_sh[k][lane].x);
+#pragma unroll
+  for (int k = 0; k < MERGE_WARPS; ++k) {
+    const float2 v = ml_sh[k][lane];
+    f[k] = v.x == -CUDART_INF_F ? 0.f : exp2f(v.x - top);
+    sum += v.y != v.y ? v.y : f[k] * v.y;
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int g = a.nq / a.nkv, r = unit.y + row;
+  T* dst = (T*)a.out + ((size_t)(unit.z + r / g) * a.nq + kvh * g + r % g) * a.hd + d0;
+  constexpr int EACH = MERGE_DIMS / MERGE_WARPS;
 #pragma unroll
-  for (int i = 0; i < MERGE_DIMS; ++i)
-    if (i < dims) dst[i] = from_float<T>(acc[i] * inv);
+  for (int i = 0; i < EACH; ++i) {
+    const int d = warp * EACH + i;
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < MERGE_WARPS; ++k) v += f[k] > 0.f ? f[k] * acc_sh[k][d][lane] : 0.f;
+    if (d < dims) dst[d] = from_float<T>(v * inv);
+  }
 }
-template <typename T, int ROWS, int KEYS>
+template <typename T, int ROWS>
 inline void launch_merge(const Args& a, int blocks, int max_rows, cudaStream_t stream) {
-  constexpr int RL = ROWS < 32 ? ROWS : 32, SPAN = 32 / RL * MERGE_WARPS * MERGE_DIMS;
-  launch_pdl(tree_merge_kernel<T, ROWS, KEYS>, dim3(blocks, (a.hd + SPAN - 1) / SPAN, ((max_rows < ROWS ? max_rows : ROWS) + RL - 1) / RL),
-             dim3(32 * MERGE_WARPS), 0, stream, a, blocks);
+  constexpr int RL = ROWS < 32 ? ROWS : 32, SPAN = 32 / RL * MERGE_DIMS;
+  launch_pdl(tree_merge_kernel<T, ROWS>, dim3(blocks, (a.hd + SPAN - 1) / SPAN, ((max_rows < ROWS ? max_rows : ROWS) + RL - 1) / RL),
+             dim3(32 * MERGE_WARPS), 0, stream, a);
+}
+
+// Lets a kernel have `bytes` of shared memory, once a device (the attribute stays with the kernel; each kernel has a `have` of its own).
+inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<int> (&have)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::atomic<int>* slot = dev < 64 ? &have[dev] : nullptr;
+  if (slot && slot->load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && slot) slot->store(bytes, std::memory_order_relaxed);
+  return e;
 }
 
 // The forms.  Each gives its blocks (C) and the rows of a unit, which size the slabs, and the keys of a tile.

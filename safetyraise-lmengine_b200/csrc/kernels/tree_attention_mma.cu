@@ -59,7 +59,9 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
   Walk<ROWS, M_KEYS> walk;
   walk.init(a, blockIdx.x, gridDim.x, blockIdx.x == 0);
   Piece w;
+  if (threadIdx.x == 0) a.part_units[blockIdx.x] = make_int4(0, 0, 0, 0);
   while (walk.next(a, w)) {
+    if (threadIdx.x == 0) leave_unit(a, walk, w);
     const Entry& x = w.x;
     const int r0 = w.block * ROWS, rows = min(ROWS, x.q_len * g - r0), tiles = w.tile_hi - w.tile_lo;
     const int* table = a.block_table + (size_t)w.e * a.table_stride;
@@ -311,10 +313,11 @@ template <int HD_MAX, int KEY_WARPS, int STAGES>
 static int run_form(const Args& a, int max_rows, int sms, cudaStream_t stream) {
   using F = MmaForm<HD_MAX, KEY_WARPS, STAGES>;
   const int smem = (int)F::smem(a.hd), blocks = mma_form(a.hd, max_rows, sms).blocks;
-  const cudaError_t e = cudaFuncSetAttribute(tree_mma_kernel<HD_MAX, KEY_WARPS, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<int> have[64];
+  const cudaError_t e = allow_smem((const void*)tree_mma_kernel<HD_MAX, KEY_WARPS, STAGES>, smem, have);
   if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", smem);
   launch_pdl(tree_mma_kernel<HD_MAX, KEY_WARPS, STAGES>, dim3(blocks), dim3(M_THREADS), smem, stream, a);
-  launch_merge<bf16, F::ROWS, M_KEYS>(a, blocks, max_rows, stream);
+  launch_merge<bf16, F::ROWS>(a, blocks, max_rows, stream);
   return launched();
 }
 // Stages: as many as leave room for another block on the SM.

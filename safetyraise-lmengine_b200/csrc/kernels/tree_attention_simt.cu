@@ -38,7 +38,9 @@ __global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const __grid_const
   Walk<S_ROWS, S_KEYS> walk;
   walk.init(a, blockIdx.x, gridDim.x, blockIdx.x == 0);
   Piece w;
+  if (threadIdx.x == 0) a.part_units[blockIdx.x] = make_int4(0, 0, 0, 0);
   while (walk.next(a, w)) {
+    if (threadIdx.x == 0) leave_unit(a, walk, w);
     const Entry& x = w.x;
     const int rows = min(S_ROWS, x.q_len * g - w.block * S_ROWS), r0 = w.block * S_ROWS;
     const int* table = a.block_table + (size_t)w.e * a.table_stride;
@@ -187,10 +189,11 @@ Form simt_form(int hd, int sms) { return Form{(hd <= 64 ? 4 : hd <= 128 ? 2 : 1)
 template <typename T, int DIMS, bool COPY>
 static int run_form(const Args& a, int max_rows, int sms, cudaStream_t stream) {
   const int smem = (int)simt_smem(a.hd), blocks = simt_form(a.hd, sms).blocks;
-  const cudaError_t e = cudaFuncSetAttribute(tree_simt_kernel<T, DIMS, COPY>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<int> have[64];
+  const cudaError_t e = allow_smem((const void*)tree_simt_kernel<T, DIMS, COPY>, smem, have);
   if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", smem);
   launch_pdl(tree_simt_kernel<T, DIMS, COPY>, dim3(blocks), dim3(S_THREADS), smem, stream, a);
-  launch_merge<T, S_ROWS, S_KEYS>(a, blocks, max_rows, stream);
+  launch_merge<T, S_ROWS>(a, blocks, max_rows, stream);
   return launched();
 }
 template <typename T, bool COPY>

@@ -34,6 +34,11 @@ struct TmaForm {
   static constexpr int SMEM = TILE * (1 + 2 * STAGES) + 1024 + (4 * STAGES + 7) * 8;
 };
 
+__device__ __forceinline__ bool elected() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
 // Scores of keys that the row does not see become -inf (the score scale is positive): a weight of zero.
 __device__ __forceinline__ void mask_row(Row& r, const uint32_t (&bits)[4]) {
   auto part = [&](uint32_t (&v)[32], uint32_t b) {
@@ -153,54 +158,66 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     __syncwarp();
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
+    // The whole warp goes through the same steps and one elected lane issues: the operands then are the warp's, and an issue costs no
+    // moves between register files (a loop that one lane alone goes through: 144 cycles an MMA, where it takes 64).
     const uint32_t idesc_s = umma_idesc(T_KEYS, false), idesc_o = umma_idesc(HD, true);
     // descriptors: the start address sits in the low bits, in units of 16 bytes, so a k-step is an addition
     const uint64_t q_desc = umma_desc(s32(q_t), 0, 1024), k_desc = umma_desc(s32(k_t), 0, 1024);
     const uint64_t v_desc = umma_desc(s32(v_t), T_KEYS * 128, 1024);
-    int k = 0, piece = 0;
-    uint32_t done[2] = {0, 0};                     // tiles of either stream so far
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const bool issues = elected();
+    int s_k = 0, s_v = 0, piece = 0;               // ring stages of the next keys and values, pieces so far
+    uint32_t k_phase = 0, v_phase = 0, p_phase = 0;        // the waits' parities, a bit a stream in the last
     bool ok = true;
     Piece w;
-    while (walk.next(a, w)) {                      // (the whole warp walks, one lane issues)
-      if (lane == 0 && ok) {
-        const int tiles = w.tile_hi - w.tile_lo;
-        auto issue_s = [&](int t) {                // S_i = Q . K_t^T
-          const int s = (k + t) % STAGES, i = t & 1;
-          ok = ok && mbar_wait(&k_full[s], ((k + t) / STAGES) & 1, a.err_flag, 83);
-          if (!ok) return;
-          fence_after();
-          const uint64_t kd = k_desc + (uint64_t)(s * (TILE >> 4));
+    if (lane == 0) a.part_units[blockIdx.x] = make_int4(0, 0, 0, 0);
+    while (walk.next(a, w)) {
+      if (lane == 0) leave_unit(a, walk, w);
+      const int tiles = __shfl_sync(0xffffffffu, w.tile_hi - w.tile_lo, 0);
+      auto issue_s = [&](int i) {                  // S_i = Q . K^T of the next keys
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&k_full[s_k], k_phase, a.err_flag, 83));
+        if (!ok) return;
+        fence_after();
+        const uint64_t kd = k_desc + (uint64_t)(s_k * (TILE >> 4));
+        if (issues) {
 #pragma unroll
           for (int ks = 0; ks < HD / 16; ++ks) {
             const uint32_t off = ((ks >> 2) * (T_KEYS * 128) + (ks & 3) * 32) >> 4;      // panel, then 32 bytes a k-step
-            umma_bf16(tmem + i * 128, q_desc + off, kd + off, idesc_s, ks != 0);
+            umma_bf16(tm + i * 128, q_desc + off, kd + off, idesc_s, ks != 0);
           }
           umma_commit(&s_full[i]);
-          umma_commit(&k_empty[s]);
-        };
-        ok = mbar_wait(q_full, piece & 1, a.err_flag, 84);
-        if (ok) fence_after();
-        if (ok) issue_s(0);
-        if (ok && tiles > 1) issue_s(1);
-        for (int t = 0; t < tiles && ok; ++t) {
-          const int s = (k + t) % STAGES, i = t & 1;
-          ok = mbar_wait(&v_full[s], ((k + t) / STAGES) & 1, a.err_flag, 85) && mbar_wait(&p_ready[i], done[i] & 1, a.err_flag, 86);
-          if (!ok) break;
-          ++done[i];
-          fence_after();
-          const uint64_t vd = v_desc + (uint64_t)(s * (TILE >> 4));
-          const uint32_t d = tmem + 256 + i * 128, p = tmem + i * 128;
+          umma_commit(&k_empty[s_k]);
+        }
+        __syncwarp();
+        if (++s_k == STAGES) s_k = 0, k_phase ^= 1;
+      };
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(q_full, piece & 1, a.err_flag, 84));
+      ++piece;
+      if (!ok) break;
+      fence_after();
+      issue_s(0);
+      if (tiles > 1) issue_s(1);
+      for (int t = 0; t < tiles && ok; ++t) {
+        const int i = t & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&v_full[s_v], v_phase, a.err_flag, 85) &&
+                                         mbar_wait(&p_ready[i], (p_phase >> i) & 1, a.err_flag, 86));
+        if (!ok) break;
+        p_phase ^= 1u << i;
+        fence_after();
+        const uint64_t vd = v_desc + (uint64_t)(s_v * (TILE >> 4));
+        const uint32_t d = tm + 256 + i * 128, p = tm + i * 128;
+        if (issues) {
 #pragma unroll
           for (int kk = 0; kk < T_KEYS / 16; ++kk)   // 16 keys: 8 columns of pairs, 2048 bytes of values
             umma_bf16_ts(d, p + kk * 8, vd + kk * (2048 >> 4), idesc_o, t > 1 || kk > 0);
           umma_commit(&o_done[i]);
-          umma_commit(&v_empty[s]);
-          if (t + 2 < tiles) issue_s(t + 2);
+          umma_commit(&v_empty[s_v]);
         }
-        k += tiles;
-        ++piece;
+        __syncwarp();
+        if (++s_v == STAGES) s_v = 0, v_phase ^= 1;
+        if (t + 2 < tiles) issue_s(i);
       }
-      __syncwarp();
+      if (!ok) break;
     }
   } else {
     // ---------------- softmax: a thread a row ----------------
@@ -414,10 +431,11 @@ static int run_form(const Args& a, int max_rows, int sms, cudaStream_t stream) {
   CUtensorMap mk, mv;
   if (rows > 0x7fffffff || !tensor_map(&mk, a.k_cache, rows, HD, box_rows) || !tensor_map(&mv, a.v_cache, rows, HD, box_rows))
     return refuse(ST_BAD_SIZE, "tree_attention: the caches of %lld rows of %d cannot be mapped", rows, HD);
-  const cudaError_t e = cudaFuncSetAttribute(tree_tcgen05_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, TmaForm<HD>::SMEM);
+  static std::atomic<int> have[64];
+  const cudaError_t e = allow_smem((const void*)tree_tcgen05_kernel<HD>, TmaForm<HD>::SMEM, have);
   if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", TmaForm<HD>::SMEM);
   launch_pdl(tree_tcgen05_kernel<HD>, dim3(sms), dim3(T_THREADS), TmaForm<HD>::SMEM, stream, mk, mv, a);
-  launch_merge<bf16, T_ROWS, T_KEYS>(a, sms, max_rows, stream);
+  launch_merge<bf16, T_ROWS>(a, sms, max_rows, stream);
   return launched();
 }
 int run_tcgen05(const Args& a, int max_rows, int sms, cudaStream_t stream) {

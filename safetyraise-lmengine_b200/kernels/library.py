@@ -835,19 +835,47 @@ class KernelLibrary:
                                       nq, nkv, hd, page_size, scale, window)
 
     # ---- drafted tokens, pages of the cache ------------------------------------------------
-    @staticmethod
-    def _here(what, *tensors):
-        """Every tensor (None: not given) lies on the current device: a launch goes to that device's stream."""
-        here = _CURRENT_DEVICE() if _CURRENT_DEVICE is not None else torch.cuda.current_device()
-        for t in tensors:
-            if t is not None and t.get_device() != here:
-                raise ShapeError(f"{what}: a tensor on {t.device}, the current device is cuda:{here}")
+    # These calls take a few microseconds of the device's time each, so the host's share counts: argument types are
+    # declared once and numbers passed as they are (a conversion object each: 24 us a call of tree_attention, 10 now).
+    _INT, _LONG, _AT, _FLOAT = C.c_int, C.c_longlong, C.c_void_p, C.c_float
+    _DRAFT_ENTRIES = {
+        "srlm_draft_tree": [_AT] * 5 + [_INT] * 4 + [_AT] * 2,
+        "srlm_tree_attention": [_AT] * 4 + [_INT, _LONG, _AT, _INT] + [_AT] * 3 + [_INT, _AT] + [_INT] * 6 + [_FLOAT, _INT, _INT, _AT, _INT, _AT, _AT],
+        "srlm_tree_attention_workspace": [_INT] * 7,
+        "srlm_accept_drafts": [_AT] * 4 + [_INT] * 2 + [_AT, _INT] + [_AT] * 4,
+        "srlm_keep_drafts": [_AT, _LONG, _LONG, _INT, _INT, _LONG, _AT, _INT] + [_AT] * 3 + [_INT, _AT, _INT, _AT, _AT],
+        "srlm_copy_pages": [_AT, _LONG, _LONG, _LONG, _AT, _AT, _INT, _INT, _AT],
+    }
+
+    def _entry(self, name):
+        entries = self.__dict__.setdefault("_draft_entries", {})
+        if name not in entries:
+            fn = getattr(self.lib, name)
+            fn.argtypes = self._DRAFT_ENTRIES[name]
+            fn.restype = C.c_longlong if name.endswith("_workspace") else C.c_int
+            entries[name] = fn
+        return entries[name]
 
     @staticmethod
-    def _ints(what, **tensors):
-        for name, (t, shape) in tensors.items():
-            if t.dtype != torch.int32 or tuple(t.shape) != shape:
-                raise ShapeError(f"{what}: {name} is int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    def _at(what, name, t, shape, dtype, here):
+        """The address of a contiguous tensor of this shape and type on the current device (a launch goes to that device's
+        stream); anything else is refused."""
+        if t.dtype is dtype and t.shape == shape and t.get_device() == here and t.is_contiguous():
+            return t.data_ptr()
+        if not t.is_cuda:
+            raise Unavailable("kernels take CUDA tensors only; there is no CPU path")
+        if t.get_device() != here:
+            raise ShapeError(f"{what}: {name} lies on {t.device}, the current device is cuda:{here}")
+        raise ShapeError(f"{what}: {name} is a contiguous {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}"
+                         f"{'' if t.is_contiguous() else ', not contiguous'}")
+
+    @staticmethod
+    def _here():
+        return _CURRENT_DEVICE() if _CURRENT_DEVICE is not None else torch.cuda.current_device()
+
+    @staticmethod
+    def _raw_stream(here):
+        return _RAW_STREAM(here) if _RAW_STREAM is not None else torch.cuda.current_stream().cuda_stream
 
     def draft_tree(self, parents, cu_q, kv_lens, positions, mask, window=0):
         """What each drafted token of a batch sees of its entry's, from the tokens' parents.
@@ -859,15 +887,18 @@ class KernelLibrary:
         window - 1 above it.  words * 32 is at least any entry's number of tokens.  A parent that does not stand before
         its child counts as none and raises the error word, as do lengths that contradict one another (such an entry is
         left out)."""
+        what, i32, here = "draft_tree", torch.int32, self._here()
         T, n = parents.shape[0], kv_lens.shape[0]
         if mask.dim() != 2 or window < 0:
             raise ShapeError(f"draft_tree: mask {list(mask.shape)} is [tokens, words], window {window} at least 0")
-        self._ints("draft_tree", parents=(parents, (T,)), cu_q=(cu_q, (n + 1,)), kv_lens=(kv_lens, (n,)),
-                   positions=(positions, (T,)), mask=(mask, (T, mask.shape[1])))
-        args = (_ptr(parents), _ptr(cu_q), _ptr(kv_lens), _ptr(positions), _ptr(mask))
-        self._here("draft_tree", parents, cu_q, kv_lens, positions, mask)
-        self._check(self.lib.srlm_draft_tree(*args, C.c_int(mask.shape[1]), C.c_int(n), C.c_int(T), C.c_int(window),
-                                             _ptr(self._gemm_state(parents.device)[1]), _stream()), "draft_tree")
+        words = mask.shape[1]
+        args = (self._at(what, "parents", parents, (T,), i32, here), self._at(what, "cu_q", cu_q, (n + 1,), i32, here),
+                self._at(what, "kv_lens", kv_lens, (n,), i32, here), self._at(what, "positions", positions, positions.shape, i32, here),
+                self._at(what, "mask", mask, (positions.shape[0], words), i32, here))
+        if positions.shape[0] != T:
+            raise ShapeError(f"draft_tree: {T} parents, {positions.shape[0]} positions")
+        self._check(self._entry("srlm_draft_tree")(*args, words, n, T, window, self._gemm_state(parents.device)[1].data_ptr(),
+                                                   self._raw_stream(here)), what)
 
     def tree_attention(self, q, k_cache, v_cache, out, block_table, cu_q, kv_lens, mask, nq, nkv, hd, page_size, scale,
                        max_q_len, positions=None, window=0):
@@ -883,47 +914,37 @@ class KernelLibrary:
         tokens).  Rows of q behind cu_q[n] are not read and theirs of out are left as they are.  What stands in places
         of the cache that a token does not see never reaches its row.  A page number outside the pool, or lengths that
         contradict one another, raise the error word (such an entry's rows are left, such a page is read as page 0)."""
-        T, n = q.shape[0], kv_lens.shape[0]
-        dtype = dtype_code(q.dtype)
-        pages = k_cache.shape[0]
-        if (tuple(q.shape) != (T, nq * hd) or tuple(out.shape) != (T, nq * hd) or tuple(k_cache.shape) != (pages, nkv, page_size, hd)
-                or k_cache.shape != v_cache.shape or mask.dim() != 2 or block_table.dim() != 2):
-            raise ShapeError(f"tree_attention: q {list(q.shape)}, out {list(out.shape)}, caches {list(k_cache.shape)} and "
-                             f"{list(v_cache.shape)}, mask {list(mask.shape)}, block table {list(block_table.shape)} with nq={nq} "
-                             f"nkv={nkv} hd={hd} page_size={page_size}")
-        if q.dtype != k_cache.dtype or q.dtype != v_cache.dtype or q.dtype != out.dtype:
-            raise ShapeError(f"tree_attention: q {q.dtype}, caches {k_cache.dtype} and {v_cache.dtype}, out {out.dtype}: one type")
-        self._ints("tree_attention", block_table=(block_table, (n, block_table.shape[1])), cu_q=(cu_q, (n + 1,)),
-                   kv_lens=(kv_lens, (n,)), mask=(mask, (T, mask.shape[1])))
-        if positions is not None:
-            self._ints("tree_attention", positions=(positions, (T,)))
+        what, i32, here, dt = "tree_attention", torch.int32, self._here(), q.dtype
+        T, n, pages = q.shape[0], kv_lens.shape[0], k_cache.shape[0]
+        code = dtype_code(dt)
+        if mask.dim() != 2 or block_table.dim() != 2:
+            raise ShapeError(f"tree_attention: mask {list(mask.shape)} is [tokens, words], block table {list(block_table.shape)} "
+                             f"[entries, pages]")
+        words, width = mask.shape[1], block_table.shape[1]
+        rows, cache = (T, nq * hd), (pages, nkv, page_size, hd)
+        args = (self._at(what, "q", q, rows, dt, here), self._at(what, "k_cache", k_cache, cache, dt, here),
+                self._at(what, "v_cache", v_cache, cache, dt, here), self._at(what, "out", out, rows, dt, here))
+        ints = (self._at(what, "block_table", block_table, (n, width), i32, here), width, self._at(what, "cu_q", cu_q, (n + 1,), i32, here),
+                self._at(what, "kv_lens", kv_lens, (n,), i32, here), self._at(what, "mask", mask, (T, words), i32, here), words,
+                None if positions is None else self._at(what, "positions", positions, (T,), i32, here))
         if T == 0 or n == 0:
             return
-        if max_q_len > 32 * mask.shape[1]:
-            raise ShapeError(f"tree_attention: {mask.shape[1]} words of a mask are too few for {max_q_len} tokens")
-        args = (_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out))
-        ints = (_ptr(block_table), C.c_int(block_table.shape[1]), _ptr(cu_q), _ptr(kv_lens), _ptr(mask), C.c_int(mask.shape[1]),
-                _ptr(positions))
-        self._here("tree_attention", q, k_cache, v_cache, out, block_table, cu_q, kv_lens, mask, positions)
+        if max_q_len > 32 * words:
+            raise ShapeError(f"tree_attention: {words} words of a mask are too few for {max_q_len} tokens")
         sms = self.sm_count(q.device)
-        words = self._tree_words(dtype, nq, nkv, hd, page_size, max_q_len, sms)
-        # of this call alone: calls on several streams, and graphs recorded apart, share nothing
-        work = torch.empty(words, dtype=torch.float32, device=q.device)
-        self._check(self.lib.srlm_tree_attention(
-            *args, C.c_int(dtype), C.c_longlong(pages), *ints, C.c_int(n), C.c_int(T), C.c_int(nq), C.c_int(nkv), C.c_int(hd),
-            C.c_int(page_size), C.c_float(scale), C.c_int(window), C.c_int(max_q_len), _ptr(work), C.c_int(sms),
-            _ptr(self._gemm_state(q.device)[1]), _stream()), "tree_attention")
-        self.launches += 1               # the kernel that adds the shares
-
-    def _tree_words(self, *sizes) -> int:
-        words = self.__dict__.setdefault("_tree_work", {}).get(sizes)
-        if words is None:
-            self.lib.srlm_tree_attention_workspace.restype = C.c_longlong
-            words = self.lib.srlm_tree_attention_workspace(*(C.c_int(s) for s in sizes))
-            if words < 0:
+        sizes = (code, nq, nkv, hd, page_size, max_q_len, sms)
+        need = self.__dict__.setdefault("_tree_work", {}).get(sizes)
+        if need is None:
+            need = self._entry("srlm_tree_attention_workspace")(*sizes)
+            if need < 0:
                 raise ShapeError(f"tree_attention refused: {self.lib.srlm_last_error().decode(errors='replace')}")
-            self._tree_work[sizes] = words
-        return words
+            self._tree_work[sizes] = need
+        # of this call alone: calls on several streams, and graphs recorded apart, share nothing
+        work = q.new_empty(need, dtype=torch.float32)
+        self._check(self._entry("srlm_tree_attention")(
+            *args, code, pages, *ints, n, T, nq, nkv, hd, page_size, scale, window, max_q_len, work.data_ptr(), sms,
+            self._gemm_state(q.device)[1].data_ptr(), self._raw_stream(here)), what)
+        self.launches += 1               # the kernel that adds the shares
 
     def accept_drafts(self, tokens, parents, targets, cu_q, path, count, next_token):
         """Follows the model's own choice down each entry's tree of drafted tokens.
@@ -933,22 +954,25 @@ class KernelLibrary:
         is the target of the token before, and on, until no child is, or path is full.  path int32 [n, room]: the
         followed tokens' places in their entry, -1 behind them; count int32 [n]: how many; next_token int32 [n]: the target
         of the last.  An entry without tokens has a count of 0 and -1."""
+        what, i32, here = "accept_drafts", torch.int32, self._here()
         T, n = tokens.shape[0], count.shape[0]
         if path.dim() != 2 or path.shape[1] < 1:
             raise ShapeError(f"accept_drafts: path {list(path.shape)} has no room")
-        self._ints("accept_drafts", tokens=(tokens, (T,)), parents=(parents, (T,)), targets=(targets, (T,)), cu_q=(cu_q, (n + 1,)),
-                   path=(path, (n, path.shape[1])), count=(count, (n,)), next_token=(next_token, (n,)))
-        args = (_ptr(tokens), _ptr(parents), _ptr(targets), _ptr(cu_q))
-        outs = (_ptr(path), C.c_int(path.shape[1]), _ptr(count), _ptr(next_token))
-        self._here("accept_drafts", tokens, parents, targets, cu_q, path, count, next_token)
-        self._check(self.lib.srlm_accept_drafts(*args, C.c_int(n), C.c_int(T), *outs, _ptr(self._gemm_state(cu_q.device)[1]),
-                                                _stream()), "accept_drafts")
+        room = path.shape[1]
+        args = (self._at(what, "tokens", tokens, (T,), i32, here), self._at(what, "parents", parents, (T,), i32, here),
+                self._at(what, "targets", targets, (T,), i32, here), self._at(what, "cu_q", cu_q, (n + 1,), i32, here), n, T,
+                self._at(what, "path", path, (n, room), i32, here), room, self._at(what, "count", count, (n,), i32, here),
+                self._at(what, "next_token", next_token, (n,), i32, here))
+        self._check(self._entry("srlm_accept_drafts")(*args, self._gemm_state(cu_q.device)[1].data_ptr(), self._raw_stream(here)), what)
 
-    def _page_pool(self, what, pool):
-        """(slabs, pages) of a pool [.., pages, kv heads, page size, head size]: what stands before the pages are its slabs."""
-        if pool.dim() < 4 or pool.numel() == 0:
-            raise ShapeError(f"{what}: a pool is [.., pages, kv heads, page size, head size], got {list(pool.shape)}")
-        return pool.numel() // (pool.shape[-4] * pool.shape[-3] * pool.shape[-2] * pool.shape[-1]), pool.shape[-4]
+    def _page_pool(self, what, pool, here):
+        """(address, slabs, pages, shape of a page) of a pool [.., pages, kv heads, page size, head size]: what stands before the
+        pages are its slabs."""
+        shape = pool.shape
+        if len(shape) < 4 or pool.numel() == 0:
+            raise ShapeError(f"{what}: a pool is [.., pages, kv heads, page size, head size], got {list(shape)}")
+        at, page = self._at(what, "pool", pool, shape, pool.dtype, here), shape[-3:]
+        return at, pool.numel() // (shape[-4] * page[0] * page[1] * page[2]), shape[-4], page
 
     def keep_drafts(self, pool, block_table, cu_q, kv_lens, path, count):
         """Moves the accepted tokens' keys and values together, in every slab of ``pool`` [.., pages, kv heads, page
@@ -957,25 +981,24 @@ class KernelLibrary:
         kv_lens as for ``tree_attention``, path and count as ``accept_drafts`` leaves them: places that rise along the
         path.  One that does not, or a page outside the pool, raises the error word and ends the entry's move there.  No
         two entries hold a page in common among their own tokens'."""
-        slabs, pages = self._page_pool("keep_drafts", pool)
+        what, i32, here = "keep_drafts", torch.int32, self._here()
+        at, slabs, pages, (nkv, page_size, hd) = self._page_pool(what, pool, here)
         n = count.shape[0]
         if path.dim() != 2 or path.shape[1] < 1 or block_table.dim() != 2:
             raise ShapeError(f"keep_drafts: path {list(path.shape)}, block table {list(block_table.shape)}")
-        self._ints("keep_drafts", block_table=(block_table, (n, block_table.shape[1])), cu_q=(cu_q, (n + 1,)), kv_lens=(kv_lens, (n,)),
-                   path=(path, (n, path.shape[1])), count=(count, (n,)))
-        args = (_ptr(pool), C.c_longlong(slabs), C.c_longlong(pages), C.c_int(pool.shape[-3]), C.c_int(pool.shape[-2]),
-                C.c_longlong(pool.shape[-1] * pool.element_size()))
-        ints = (_ptr(block_table), C.c_int(block_table.shape[1]), _ptr(cu_q), _ptr(kv_lens), _ptr(path), C.c_int(path.shape[1]),
-                _ptr(count))
-        self._here("keep_drafts", pool, block_table, cu_q, kv_lens, path, count)
-        self._check(self.lib.srlm_keep_drafts(*args, *ints, C.c_int(n), _ptr(self._gemm_state(pool.device)[1]), _stream()),
-                    "keep_drafts")
+        room, width = path.shape[1], block_table.shape[1]
+        ints = (self._at(what, "block_table", block_table, (n, width), i32, here), width, self._at(what, "cu_q", cu_q, (n + 1,), i32, here),
+                self._at(what, "kv_lens", kv_lens, (n,), i32, here), self._at(what, "path", path, (n, room), i32, here), room,
+                self._at(what, "count", count, (n,), i32, here))
+        self._check(self._entry("srlm_keep_drafts")(at, slabs, pages, nkv, page_size, hd * pool.element_size(), *ints, n,
+                                                    self._gemm_state(pool.device)[1].data_ptr(), self._raw_stream(here)), what)
 
     def copy_pages(self, pool, src, dst):
         """Page dst[i] takes what page src[i] holds, in every slab of ``pool`` [.., pages, kv heads, page size, head
         size].  src and dst are page numbers on the host (the cache manager's); a page may be copied several times, none
         is written twice, and none is both read and written."""
-        slabs, pages = self._page_pool("copy_pages", pool)
+        what, here = "copy_pages", self._here()
+        at, slabs, pages, page = self._page_pool(what, pool, here)
         numbers = []
         for x in (src, dst):
             if isinstance(x, torch.Tensor) and x.is_cuda:
@@ -986,12 +1009,9 @@ class KernelLibrary:
             numbers.append(np.ascontiguousarray(x, dtype=np.int64))
         if numbers[0].size != numbers[1].size:
             raise ShapeError(f"copy_pages: {numbers[0].size} pages to {numbers[1].size}")
-        ptr = _ptr(pool)
-        self._here("copy_pages", pool)
-        self._check(self.lib.srlm_copy_pages(
-            ptr, C.c_longlong(slabs), C.c_longlong(pages), C.c_longlong(pool.shape[-3] * pool.shape[-2] * pool.shape[-1] * pool.element_size()),
-            C.c_void_p(numbers[0].ctypes.data), C.c_void_p(numbers[1].ctypes.data), C.c_int(numbers[0].size),
-            C.c_int(self.sm_count(pool.device)), _stream()), "copy_pages")
+        self._check(self._entry("srlm_copy_pages")(
+            at, slabs, pages, page[0] * page[1] * page[2] * pool.element_size(), numbers[0].ctypes.data, numbers[1].ctypes.data,
+            numbers[0].size, self.sm_count(pool.device), self._raw_stream(here)), what)
 
     # ---- blocks that norm on both sides of a sublayer --------------------------------
     def gated_postnorm_add(self, residual, sub, gate, gate_bias, post_w, eps, next_w=None, next_eps=0.0,
