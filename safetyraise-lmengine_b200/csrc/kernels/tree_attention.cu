@@ -55,8 +55,8 @@ extern "C" int srlm_tree_attention(const void* q, const void* k_cache, const voi
     if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) % 16)
       return refuse(ST_BAD_ALIGN, "tree_attention: bfloat16 tensors start on 16-byte boundaries");
     a.least_tiles = 2;
-    return kind == TCGEN05 ? tree::run_tcgen05(a, max_rows, sms, stream) : tree::run_mma(a, max_rows, sms, stream);
+    return kind == TCGEN05 ? tree::run_tcgen05(a, sms, stream) : tree::run_mma(a, max_rows, sms, stream);
   }
   a.least_tiles = 4;
-  return tree::run_simt(a, dtype, max_rows, sms, stream);
+  return tree::run_simt(a, dtype, sms, stream);
 }

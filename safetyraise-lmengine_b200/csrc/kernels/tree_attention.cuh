@@ -19,6 +19,7 @@
 
 #include <math_constants.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "common.cuh"
@@ -50,7 +51,7 @@ struct Args {
   int* err_flag;
   float* part_o;             // slabs [2 C][hd][ROWS]: neighbouring rows side by side, as the threads that write and read them are
   float* part_ml;            // [2 C][ROWS][2]: reference maximum (log2 units), sum of weights
-  int4* part_units;          // [C]: the unit that begins in share C and goes on behind it: slabs (0: none such), first row of its
+  int4* part_units;          // [C]: the unit that begins in share C and goes on behind it: its slabs (0: none such), first row of its
                              // entry's rows, first token of the entry, KV head | rows << 16
 };
 
@@ -251,8 +252,8 @@ __device__ __noinline__ float loose_values(const Args& a, int start, int kv_len,
   return sum;
 }
 
-// What a block leaves for the merge beside its slabs, by one thread: the unit that goes on behind its share (it begins in the last
-// piece), or that there is none.
+// What a block leaves for the merge beside its slabs, by one thread: the unit that goes on behind its share, or that there is none.
+__device__ __forceinline__ void leave_no_unit(const Args& a) { a.part_units[blockIdx.x] = make_int4(0, 0, 0, 0); }
 template <int ROWS, int KEYS>
 __device__ __forceinline__ void leave_unit(const Args& a, const Walk<ROWS, KEYS>& w, const Piece& p) {
   if (!p.begins || p.ends) return;
@@ -262,79 +263,94 @@ __device__ __forceinline__ void leave_unit(const Args& a, const Walk<ROWS, KEYS>
 }
 
 // Adds the slabs of the unit that begins in share blockIdx.x and goes on behind it: out = sum_z O_z 2^(m_z - M) / sum_z l_z
-// 2^(m_z - M), M the largest reference of a slab that saw a key.  A lane has a row and MERGE_DIMS of its dimensions (of units of
-// fewer rows than lanes, a warp has several such runs); the block's warps take the slabs in turn and add up their shares in shared
-// memory, so that a row of many slabs costs a few reads one behind another.
-constexpr int MERGE_WARPS = 8, MERGE_DIMS = 16;
+// 2^(m_z - M), M the largest reference of a slab that saw a key; which slabs a warp adds depends on their number alone.
+// A block has 32 rows (blockIdx.y), a lane one of them and MERGE_DIMS dimensions (of units of 16 rows a warp has two such runs);
+// what warps the dimensions leave deal the slabs among themselves and add up in shared memory.  The kernel is all latency -- the
+// unit's record, the slabs, the result -- and the code of one round is what it fetches: written out for several slabs at once, or with
+// a pass of its own for the references, it took 10 us and more where this takes 3.
+constexpr int MERGE_WARPS = 32, MERGE_DIMS = 8, MERGE_TURNS = 4;
 
 template <typename T, int ROWS>
-__global__ void __launch_bounds__(32 * MERGE_WARPS) tree_merge_kernel(const __grid_constant__ Args a) {
-  constexpr int RL = ROWS < 32 ? ROWS : 32, RUNS = 32 / RL;            // rows, runs of a warp
-  __shared__ float acc_sh[MERGE_WARPS][MERGE_DIMS][32];
+__global__ void __launch_bounds__(32 * MERGE_WARPS) tree_merge_kernel(const __grid_constant__ Args a, int dim_warps, int turns) {
+  constexpr int RL = ROWS < 32 ? ROWS : 32;
+  __shared__ float acc_sh[(MERGE_WARPS - MERGE_WARPS / MERGE_TURNS) * MERGE_DIMS][32];
   __shared__ float2 ml_sh[MERGE_WARPS][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int share = blockIdx.x, row = blockIdx.z * RL + lane % RL, d0 = (blockIdx.y * RUNS + lane / RL) * MERGE_DIMS;
+  const int turn = warp / dim_warps, share = blockIdx.x, row = blockIdx.y * RL + lane % RL;
+  const int d0 = (warp % dim_warps * (32 / RL) + lane / RL) * MERGE_DIMS, dims = min(MERGE_DIMS, a.hd - d0);
   pdl_wait();
   pdl_trigger();
   const int4 unit = a.part_units[share];
   const int slabs = unit.x, kvh = unit.w & 0xffff, rows = unit.w >> 16;
-  if (slabs == 0 || blockIdx.z * RL >= rows) return;
-  const int dims = min(MERGE_DIMS, a.hd - d0);
-  const bool there = row < rows && dims > 0;
+  if (slabs == 0 || (int)blockIdx.y * RL >= rows) return;
   float acc[MERGE_DIMS], M = -CUDART_INF_F, L = 0.f;
 #pragma unroll
   for (int i = 0; i < MERGE_DIMS; ++i) acc[i] = 0.f;
-  if (there)
-    for (int z = warp; z < slabs; z += MERGE_WARPS) {
-      const size_t slab = slab_of(share + z, z == 0);
-      const float2 v = *reinterpret_cast<const float2*>(a.part_ml + (slab * ROWS + row) * 2);
-      const float* src = a.part_o + (slab * a.hd + d0) * ROWS + row;
-      float o[MERGE_DIMS];
+#pragma unroll 2
+  for (int z = row < rows ? turn : slabs; z < slabs; z += turns) {
+    const size_t slab = slab_of(share + z, z == 0);
+    const float2 v = *reinterpret_cast<const float2*>(a.part_ml + (slab * ROWS + row) * 2);
+    const float* src = a.part_o + (slab * a.hd + d0) * ROWS + row;
+    float o[MERGE_DIMS];
 #pragma unroll
-      for (int i = 0; i < MERGE_DIMS; ++i) o[i] = i < dims ? src[i * ROWS] : 0.f;
-      if (v.y > 0.f) {                                                 // (a slab of no key holds nothing)
+    for (int i = 0; i < MERGE_DIMS; ++i) o[i] = i < dims ? src[i * ROWS] : 0.f;
+    if (v.y > 0.f) {                                                 // (a slab of no key holds nothing)
+      const float m_new = fmaxf(M, v.x), f = exp2f(v.x - m_new), old = exp2f(M - m_new);
+      M = m_new;
+      L = L * old + f * v.y;
+#pragma unroll
+      for (int i = 0; i < MERGE_DIMS; ++i) acc[i] = acc[i] * old + f * o[i];
+    } else if (v.y != v.y) {
+      L = v.y;                                                       // (a score that was no number makes the row none)
+    }
+  }
+  if (turns > 1) {
+    if (turn > 0) {
+      ml_sh[warp][lane] = make_float2(M, L);
+#pragma unroll
+      for (int i = 0; i < MERGE_DIMS; ++i) acc_sh[(warp - dim_warps) * MERGE_DIMS + i][lane] = acc[i];
+    }
+    __syncthreads();
+    if (turn > 0) return;
+#pragma unroll 1
+    for (int w = warp + dim_warps; w < turns * dim_warps; w += dim_warps) {
+      const float2 v = ml_sh[w][lane];
+      if (v.y > 0.f) {
         const float m_new = fmaxf(M, v.x), f = exp2f(v.x - m_new), old = exp2f(M - m_new);
         M = m_new;
         L = L * old + f * v.y;
 #pragma unroll
-        for (int i = 0; i < MERGE_DIMS; ++i) acc[i] = acc[i] * old + f * o[i];
+        for (int i = 0; i < MERGE_DIMS; ++i) acc[i] = acc[i] * old + f * acc_sh[(w - dim_warps) * MERGE_DIMS + i][lane];
       } else if (v.y != v.y) {
-        L = v.y;                                                       // (a score that was no number makes the row none)
+        L = v.y;
       }
     }
-  ml_sh[warp][lane] = make_float2(M, L);
-#pragma unroll
-  for (int i = 0; i < MERGE_DIMS; ++i) acc_sh[warp][i][lane] = acc[i];
-  __syncthreads();
-  if (!there) return;
-  // each warp writes its part of the dimensions
-  float f[MERGE_WARPS], top = -CUDART_INF_F, sum = 0.f;
-#pragma unroll
-  for (int k = 0; k < MERGE_WARPS; ++k) top = fmaxf(top, ml_sh[k][lane].x);
-#pragma unroll
-  for (int k = 0; k < MERGE_WARPS; ++k) {
-    const float2 v = ml_sh[k][lane];
-    f[k] = v.x == -CUDART_INF_F ? 0.f : exp2f(v.x - top);
-    sum += v.y != v.y ? v.y : f[k] * v.y;
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (row >= rows || dims <= 0) return;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
   const int g = a.nq / a.nkv, r = unit.y + row;
   T* dst = (T*)a.out + ((size_t)(unit.z + r / g) * a.nq + kvh * g + r % g) * a.hd + d0;
-  constexpr int EACH = MERGE_DIMS / MERGE_WARPS;
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    const int d = warp * EACH + i;
-    float v = 0.f;
+  for (int i = 0; i < MERGE_DIMS; ++i) acc[i] *= inv;
+  if constexpr (sizeof(T) == 2) {
+    if (a.hd % MERGE_DIMS == 0 && (uintptr_t)a.out % 16 == 0) {
+      __nv_bfloat162 p[MERGE_DIMS / 2];
 #pragma unroll
-    for (int k = 0; k < MERGE_WARPS; ++k) v += f[k] > 0.f ? f[k] * acc_sh[k][d][lane] : 0.f;
-    if (d < dims) dst[d] = from_float<T>(v * inv);
+      for (int i = 0; i < MERGE_DIMS / 2; ++i) p[i] = __floats2bfloat162_rn(acc[2 * i], acc[2 * i + 1]);
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(p);
+      return;
+    }
   }
+#pragma unroll
+  for (int i = 0; i < MERGE_DIMS; ++i)
+    if (i < dims) dst[i] = from_float<T>(acc[i]);
 }
 template <typename T, int ROWS>
-inline void launch_merge(const Args& a, int blocks, int max_rows, cudaStream_t stream) {
+inline void launch_merge(const Args& a, int blocks, cudaStream_t stream) {
   constexpr int RL = ROWS < 32 ? ROWS : 32, SPAN = 32 / RL * MERGE_DIMS;
-  launch_pdl(tree_merge_kernel<T, ROWS>, dim3(blocks, (a.hd + SPAN - 1) / SPAN, ((max_rows < ROWS ? max_rows : ROWS) + RL - 1) / RL),
-             dim3(32 * MERGE_WARPS), 0, stream, a);
+  const int dim_warps = (a.hd + SPAN - 1) / SPAN, turns = std::min(MERGE_TURNS, MERGE_WARPS / dim_warps);
+  const int max_rows = std::min(a.max_q_len * (a.nq / a.nkv), ROWS);
+  launch_pdl(tree_merge_kernel<T, ROWS>, dim3(blocks, (max_rows + RL - 1) / RL), dim3(32 * dim_warps * turns), 0, stream, a, dim_warps, turns);
 }
 
 // Lets a kernel have `bytes` of shared memory, once a device (the attribute stays with the kernel; each kernel has a `have` of its own).
@@ -354,13 +370,13 @@ struct Form {
   int blocks, rows, keys;
 };
 Form simt_form(int hd, int sms);
-int run_simt(const Args& a, int dtype, int max_rows, int sms, cudaStream_t stream);
+int run_simt(const Args& a, int dtype, int sms, cudaStream_t stream);
 bool mma_takes(int hd);                            // bfloat16
 Form mma_form(int hd, int max_rows, int sms);
 int run_mma(const Args& a, int max_rows, int sms, cudaStream_t stream);
 bool tcgen05_takes(int hd, int page_size);         // bfloat16
 Form tcgen05_form(int sms);
-int run_tcgen05(const Args& a, int max_rows, int sms, cudaStream_t stream);
+int run_tcgen05(const Args& a, int sms, cudaStream_t stream);
 
 }  // namespace tree
 }  // namespace srlm

@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
   Walk<ROWS, M_KEYS> walk;
   walk.init(a, blockIdx.x, gridDim.x, blockIdx.x == 0);
   Piece w;
-  if (threadIdx.x == 0) a.part_units[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (threadIdx.x == 0) leave_no_unit(a);
   while (walk.next(a, w)) {
     if (threadIdx.x == 0) leave_unit(a, walk, w);
     const Entry& x = w.x;
@@ -310,23 +310,24 @@ bool mma_takes(int hd) { return hd % 16 == 0 && hd <= 256; }
 Form mma_form(int hd, int max_rows, int sms) { return Form{blocks_per_sm(hd) * sms, 64 / key_warps(max_rows), M_KEYS}; }
 
 template <int HD_MAX, int KEY_WARPS, int STAGES>
-static int run_form(const Args& a, int max_rows, int sms, cudaStream_t stream) {
+static int run_form(const Args& a, int blocks, cudaStream_t stream) {
   using F = MmaForm<HD_MAX, KEY_WARPS, STAGES>;
-  const int smem = (int)F::smem(a.hd), blocks = mma_form(a.hd, max_rows, sms).blocks;
+  const int smem = (int)F::smem(a.hd);
   static std::atomic<int> have[64];
   const cudaError_t e = allow_smem((const void*)tree_mma_kernel<HD_MAX, KEY_WARPS, STAGES>, smem, have);
   if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", smem);
   launch_pdl(tree_mma_kernel<HD_MAX, KEY_WARPS, STAGES>, dim3(blocks), dim3(M_THREADS), smem, stream, a);
-  launch_merge<bf16, F::ROWS>(a, blocks, max_rows, stream);
+  launch_merge<bf16, F::ROWS>(a, blocks, stream);
   return launched();
 }
 // Stages: as many as leave room for another block on the SM.
 template <int HD_MAX, int STAGES, int STAGES_ROWS>
 static int run_rows(const Args& a, int max_rows, int sms, cudaStream_t stream) {
+  const int blocks = mma_form(a.hd, max_rows, sms).blocks;
   switch (key_warps(max_rows)) {
-    case 4: return run_form<HD_MAX, 4, STAGES>(a, max_rows, sms, stream);
-    case 2: return run_form<HD_MAX, 2, STAGES>(a, max_rows, sms, stream);
-    default: return run_form<HD_MAX, 1, STAGES_ROWS>(a, max_rows, sms, stream);
+    case 4: return run_form<HD_MAX, 4, STAGES>(a, blocks, stream);
+    case 2: return run_form<HD_MAX, 2, STAGES>(a, blocks, stream);
+    default: return run_form<HD_MAX, 1, STAGES_ROWS>(a, blocks, stream);
   }
 }
 int run_mma(const Args& a, int max_rows, int sms, cudaStream_t stream) {

@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const __grid_const
   Walk<S_ROWS, S_KEYS> walk;
   walk.init(a, blockIdx.x, gridDim.x, blockIdx.x == 0);
   Piece w;
-  if (threadIdx.x == 0) a.part_units[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (threadIdx.x == 0) leave_no_unit(a);
   while (walk.next(a, w)) {
     if (threadIdx.x == 0) leave_unit(a, walk, w);
     const Entry& x = w.x;
@@ -187,25 +187,25 @@ __global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const __grid_const
 Form simt_form(int hd, int sms) { return Form{(hd <= 64 ? 4 : hd <= 128 ? 2 : 1) * sms, S_ROWS, S_KEYS}; }
 
 template <typename T, int DIMS, bool COPY>
-static int run_form(const Args& a, int max_rows, int sms, cudaStream_t stream) {
+static int run_form(const Args& a, int sms, cudaStream_t stream) {
   const int smem = (int)simt_smem(a.hd), blocks = simt_form(a.hd, sms).blocks;
   static std::atomic<int> have[64];
   const cudaError_t e = allow_smem((const void*)tree_simt_kernel<T, DIMS, COPY>, smem, have);
   if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", smem);
   launch_pdl(tree_simt_kernel<T, DIMS, COPY>, dim3(blocks), dim3(S_THREADS), smem, stream, a);
-  launch_merge<T, S_ROWS>(a, blocks, max_rows, stream);
+  launch_merge<T, S_ROWS>(a, blocks, stream);
   return launched();
 }
 template <typename T, bool COPY>
-static int run_dims(const Args& a, int max_rows, int sms, cudaStream_t stream) {
-  if (a.hd <= 64) return run_form<T, 2, COPY>(a, max_rows, sms, stream);
-  if (a.hd <= 128) return run_form<T, 4, COPY>(a, max_rows, sms, stream);
-  return run_form<T, 8, COPY>(a, max_rows, sms, stream);
+static int run_dims(const Args& a, int sms, cudaStream_t stream) {
+  if (a.hd <= 64) return run_form<T, 2, COPY>(a, sms, stream);
+  if (a.hd <= 128) return run_form<T, 4, COPY>(a, sms, stream);
+  return run_form<T, 8, COPY>(a, sms, stream);
 }
-int run_simt(const Args& a, int dtype, int max_rows, int sms, cudaStream_t stream) {
-  if (dtype == DT_BF16) return run_dims<bf16, false>(a, max_rows, sms, stream);
-  if (a.hd % 4 == 0 && ((uintptr_t)a.k_cache | (uintptr_t)a.v_cache) % 16 == 0) return run_dims<float, true>(a, max_rows, sms, stream);
-  return run_dims<float, false>(a, max_rows, sms, stream);
+int run_simt(const Args& a, int dtype, int sms, cudaStream_t stream) {
+  if (dtype == DT_BF16) return run_dims<bf16, false>(a, sms, stream);
+  if (a.hd % 4 == 0 && ((uintptr_t)a.k_cache | (uintptr_t)a.v_cache) % 16 == 0) return run_dims<float, true>(a, sms, stream);
+  return run_dims<float, false>(a, sms, stream);
 }
 
 }  // namespace tree

@@ -170,7 +170,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     uint32_t k_phase = 0, v_phase = 0, p_phase = 0;        // the waits' parities, a bit a stream in the last
     bool ok = true;
     Piece w;
-    if (lane == 0) a.part_units[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (lane == 0) leave_no_unit(a);
     while (walk.next(a, w)) {
       if (lane == 0) leave_unit(a, walk, w);
       const int tiles = __shfl_sync(0xffffffffu, w.tile_hi - w.tile_lo, 0);
@@ -425,7 +425,7 @@ bool tcgen05_takes(int hd, int page_size) {
 Form tcgen05_form(int sms) { return Form{sms, T_ROWS, T_KEYS}; }
 
 template <int HD>
-static int run_form(const Args& a, int max_rows, int sms, cudaStream_t stream) {
+static int run_form(const Args& a, int sms, cudaStream_t stream) {
   const int box_rows = min(a.page_size, T_KEYS);
   const long long rows = (long long)a.num_pages * a.nkv * a.page_size;
   CUtensorMap mk, mv;
@@ -435,11 +435,11 @@ static int run_form(const Args& a, int max_rows, int sms, cudaStream_t stream) {
   const cudaError_t e = allow_smem((const void*)tree_tcgen05_kernel<HD>, TmaForm<HD>::SMEM, have);
   if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", TmaForm<HD>::SMEM);
   launch_pdl(tree_tcgen05_kernel<HD>, dim3(sms), dim3(T_THREADS), TmaForm<HD>::SMEM, stream, mk, mv, a);
-  launch_merge<bf16, T_ROWS>(a, sms, max_rows, stream);
+  launch_merge<bf16, T_ROWS>(a, sms, stream);
   return launched();
 }
-int run_tcgen05(const Args& a, int max_rows, int sms, cudaStream_t stream) {
-  return a.hd == 64 ? run_form<64>(a, max_rows, sms, stream) : run_form<128>(a, max_rows, sms, stream);
+int run_tcgen05(const Args& a, int sms, cudaStream_t stream) {
+  return a.hd == 64 ? run_form<64>(a, sms, stream) : run_form<128>(a, sms, stream);
 }
 
 }  // namespace tree
