@@ -6,9 +6,9 @@
 using namespace srlm;
 
 enum Kind { SIMT, MMA, TCGEN05 };
-static Kind kind_of(int dtype, int hd, int page_size, int max_rows) {
+static Kind kind_of(int dtype, int hd, int page_size) {
   if (dtype != DT_BF16 || !tree::mma_takes(hd)) return SIMT;
-  return max_rows > 16 && tree::tcgen05_takes(hd, page_size) ? TCGEN05 : MMA;
+  return tree::tcgen05_takes(hd, page_size) ? TCGEN05 : MMA;
 }
 static tree::Form form_of(Kind kind, int hd, int max_rows, int sms) {
   return kind == TCGEN05 ? tree::tcgen05_form(sms) : kind == MMA ? tree::mma_form(hd, max_rows, sms) : tree::simt_form(hd, sms);
@@ -23,7 +23,7 @@ extern "C" long long srlm_tree_attention_workspace(int dtype, int nq, int nkv, i
     return -1;
   }
   const int max_rows = max_q_len * (nq / nkv);
-  const tree::Form f = form_of(kind_of(dtype, hd, page_size, max_rows), hd, max_rows, sms);
+  const tree::Form f = form_of(kind_of(dtype, hd, page_size), hd, max_rows, sms);
   return 2ll * f.blocks * f.rows * (hd + 2) + 4ll * f.blocks;
 }
 
@@ -40,7 +40,7 @@ extern "C" int srlm_tree_attention(const void* q, const void* k_cache, const voi
     return refuse(ST_BAD_SIZE, "tree_attention: words=%d table_stride=%d num_pages=%lld window=%d scale=%g (a window needs the positions, a "
                   "scale is positive)", words, table_stride, num_pages, window, (double)scale);
   const int max_rows = max_q_len * (nq / nkv);
-  const Kind kind = kind_of(dtype, hd, page_size, max_rows);
+  const Kind kind = kind_of(dtype, hd, page_size);
   const tree::Form f = form_of(kind, hd, max_rows, sms);
   // the list of all units' tiles is counted in 31 bits
   const double units = (double)n * nkv * ((double)max_q_len * (nq / nkv) / f.rows + 1), tiles = (double)table_stride * page_size / f.keys + 1;
@@ -49,7 +49,8 @@ extern "C" int srlm_tree_attention(const void* q, const void* k_cache, const voi
                   table_stride);
   float* ml = work + 2ll * f.blocks * f.rows * hd;      // (sizes are multiples of 16 bytes)
   tree::Args a{q, k_cache, v_cache, out, block_table, table_stride, cu_q, kv_lens, mask, words, std::min(max_q_len, 32 * words), positions, n, T,
-               nq, nkv, hd, page_size, (int)num_pages, scale * 1.4426950408889634f, window, 1, err_flag, work,
+               nq, nkv, nq / nkv, hd, page_size, (int)num_pages, scale * 1.4426950408889634f,
+               2.f * hd * (dtype == DT_F32 ? 4 : 2), window, 1, err_flag, work,
                ml, reinterpret_cast<int4*>(ml + 4ll * f.blocks * f.rows)};
   if (kind != SIMT) {
     if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) % 16)

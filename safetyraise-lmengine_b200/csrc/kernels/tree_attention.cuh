@@ -9,12 +9,15 @@
 //
 // Division.  A unit is (entry, KV head, block of ROWS rows), a row being (token, head of the KV head's group); it walks its
 // entry's keys in tiles of KEYS from the first one that the window leaves anybody.  All units' tiles stand in one list, in the
-// order of entries, KV heads, blocks of rows; block c of C takes the tiles [c W / C, (c + 1) W / C) of the W, whatever units
+// order of entries, KV heads, blocks of rows; share c of C is the tiles [c W / C, (c + 1) W / C) of the W, whatever units
 // they belong to: every SM has the same number of tiles to within one, for one long request as for many ragged ones, and the
 // division needs nothing from the host (lengths may change between replays of a graph).  A unit whose tiles lie with one
 // block is written by that block; one that several share is left as unnormalised sums with their reference maximum and sum of
 // weights (a slab per block: it has at most one unit that began before it and one that goes on behind it), which
 // tree_merge_kernel adds in the order of the keys.  The sums depend on the lengths and C alone.
+// Where units of several blocks of rows read more keys than the L2 cache holds, their blocks go through the same tiles at the same
+// time, as many thread blocks side by side as the units have blocks of rows (members): the keys come from memory once and not once
+// for each (8 entries of 320 rows behind up to 32,768 keys: 380 us apart, 316 side by side).
 #pragma once
 
 #include <math_constants.h>
@@ -43,16 +46,17 @@ struct Args {
   int max_q_len;             // no entry has more tokens
   const int* positions;      // null without a window
   int n, T;                  // entries; rows of q and out
-  int nq, nkv, hd, page_size;
+  int nq, nkv, g, hd, page_size;      // g: query heads of a KV head
   int num_pages;
   float scale_log2;          // score scale times log2(e)
+  float key_bytes;           // of a key and its value in one KV head
   int window;
   int least_tiles;           // a block takes at least so many tiles
   int* err_flag;
   float* part_o;             // slabs [2 C][hd][ROWS]: neighbouring rows side by side, as the threads that write and read them are
   float* part_ml;            // [2 C][ROWS][2]: reference maximum (log2 units), sum of weights
-  int4* part_units;          // [C]: the unit that begins in share C and goes on behind it: its slabs (0: none such), first row of its
-                             // entry's rows, first token of the entry, KV head | rows << 16
+  int4* part_units;          // [C]: the unit that begins in share C and goes on behind it: its slabs (0: none such) | members << 16, first row
+                             // of its entry's rows, first token of the entry, KV head | rows << 16
 };
 
 struct Entry {
@@ -80,7 +84,7 @@ __device__ __forceinline__ Entry entry_of(const Args& a, int e, bool flag = fals
   const int first = a.window > 0 ? max(0, x.start - a.window + 1) : 0;
   x.first_tile = first / KEYS;
   x.tiles = (x.kv_len + KEYS - 1) / KEYS - x.first_tile;
-  x.blocks = (x.q_len * (a.nq / a.nkv) + ROWS - 1) / ROWS;
+  x.blocks = (x.q_len * a.g + ROWS - 1) / ROWS;
   return x;
 }
 
@@ -92,16 +96,19 @@ struct Piece {
   bool begins, ends;           // the unit's first tile, its last one, are the piece's
 };
 
+constexpr float L2_HELD = 64e6f;     // bytes of keys and values that units read one behind another still find in the L2 cache
+
 // A block's share of the list.  Every warp that calls next() walks the same pieces.  (A list is shorter than 2^31: the entry
 // point sees to it.)
 template <int ROWS, int KEYS>
 struct Walk {
   int at, end;                 // the next tile and the share's end
-  int blocks, each, more;      // blocks that have a share; of `each` tiles, the first `more` of them of one more
+  int members, member;         // thread blocks side by side on a share, each with a block of rows; 1: shares of all units' tiles
+  int each, more;              // tiles of a share; the first `more` shares have one more
   int e, base;                 // entry of the tile `at`, whose list begins at `base`
   Entry x;
 
-  __device__ __forceinline__ int weight(const Args& a, const Entry& y) const { return y.tiles * y.blocks * a.nkv; }
+  __device__ __forceinline__ int weight(const Args& a, const Entry& y) const { return y.tiles * a.nkv * (members > 1 ? 1 : y.blocks); }
   __device__ __forceinline__ int first_of(int share) const { return share * each + min(share, more); }
   // the share that holds the tile `pos`
   __device__ __forceinline__ int share_of(int pos) const {
@@ -109,25 +116,43 @@ struct Walk {
     return pos < longer ? pos / (each + 1) : more + (pos - longer) / each;
   }
 
-  // All lanes of a warp.  share: which of `blocks_there`; the entries' tiles are counted by the warp, 32 entries a turn.
-  __device__ __forceinline__ void init(const Args& a, int share, int blocks_there, bool flag) {
-    const int lane = threadIdx.x & 31;
-    int w = 0, total = 0;
+  // All lanes of a warp: the entries' tiles are counted by the warp, 32 entries a turn.
+  __device__ __forceinline__ void init(const Args& a, bool flag) {
+    const int lane = threadIdx.x & 31, there = gridDim.x;
+    Entry mine;
+    int whole = 0, single = 0, most = 0;         // tiles of all units, of one block of rows each; most blocks of rows
     for (int e0 = 0; e0 < a.n; e0 += 32) {
-      w = e0 + lane < a.n ? weight(a, entry_of<ROWS, KEYS>(a, e0 + lane, flag)) : 0;
-      total += __reduce_add_sync(0xffffffffu, w);
+      if (e0 + lane < a.n) mine = entry_of<ROWS, KEYS>(a, e0 + lane, flag);
+      else mine.tiles = mine.blocks = 0;
+      const int w = mine.tiles * a.nkv;
+      single += __reduce_add_sync(0xffffffffu, w);
+      whole += __reduce_add_sync(0xffffffffu, w * mine.blocks);
+      most = max(most, __reduce_max_sync(0xffffffffu, mine.blocks));
     }
-    blocks = min((total + a.least_tiles - 1) / a.least_tiles, blocks_there);
+    members = 1;
+    if (most > 1 && most <= 8 && (float)single * KEYS * a.key_bytes > L2_HELD) {
+      // side by side, unless blocks of rows that some entries do not have would leave a tenth of the time empty
+      const int used = there / most * most;
+      if ((float)whole * there >= 0.9f * (float)single * most * used && (float)whole >= 0.9f * (float)single * most) members = most;
+    }
+    const int total = members > 1 ? single : whole;
+    const int share = members > 1 ? blockIdx.x / members : blockIdx.x;
+    member = blockIdx.x - share * members;
+    const int shares = min((total + a.least_tiles - 1) / a.least_tiles, there / members);
     at = end = base = e = each = more = 0;
-    if (share >= blocks) return;
-    each = total / blocks;
-    more = total - each * blocks;
+    if (share >= shares) return;
+    each = total / shares;
+    more = total - each * shares;
     at = first_of(share);
     end = first_of(share + 1);
     // the entry that holds the tile
     int before = 0;
     for (int e0 = 0; e0 < a.n; e0 += 32) {
-      if (a.n > 32) w = e0 + lane < a.n ? weight(a, entry_of<ROWS, KEYS>(a, e0 + lane)) : 0;
+      if (a.n > 32) {
+        if (e0 + lane < a.n) mine = entry_of<ROWS, KEYS>(a, e0 + lane);
+        else mine.tiles = mine.blocks = 0;
+      }
+      const int w = weight(a, mine);
       int upto = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -146,27 +171,30 @@ struct Walk {
     x = entry_of<ROWS, KEYS>(a, e);
   }
   __device__ __forceinline__ bool next(const Args& a, Piece& p) {
-    if (at >= end) return false;
-    while (at - base >= weight(a, x)) {
-      base += weight(a, x);
-      x = entry_of<ROWS, KEYS>(a, ++e);          // (at is below the total: such an entry is there)
+    while (at < end) {
+      while (at - base >= weight(a, x)) {
+        base += weight(a, x);
+        x = entry_of<ROWS, KEYS>(a, ++e);        // (at is below the total: such an entry is there)
+      }
+      const int unit = (at - base) / x.tiles, t = at - base - unit * x.tiles, count = min(end - at, x.tiles - t);
+      at += count;
+      if (member >= x.blocks) continue;          // a block of rows that this entry does not have
+      p.x = x;
+      p.e = e;
+      p.kvh = members > 1 ? unit : unit / x.blocks;
+      p.block = members > 1 ? member : unit - p.kvh * x.blocks;
+      p.tile_lo = x.first_tile + t;
+      p.tile_hi = p.tile_lo + count;
+      p.begins = t == 0;
+      p.ends = t + count == x.tiles;
+      return true;
     }
-    const int unit = (at - base) / x.tiles, t = at - base - unit * x.tiles, count = min(end - at, x.tiles - t);
-    p.x = x;
-    p.e = e;
-    p.kvh = unit / x.blocks;
-    p.block = unit - p.kvh * x.blocks;
-    p.tile_lo = x.first_tile + t;
-    p.tile_hi = p.tile_lo + count;
-    p.begins = t == 0;
-    p.ends = t + count == x.tiles;
-    at += count;
-    return true;
+    return false;
   }
 };
 
-// The slab of a piece that is not a whole unit.
-__device__ __forceinline__ size_t slab_of(int share, bool begins) { return 2 * (size_t)share + (begins ? 1 : 0); }
+// The slab of a block's piece that is not a whole unit.
+__device__ __forceinline__ size_t slab_of(int block, bool begins) { return 2 * (size_t)block + (begins ? 1 : 0); }
 
 // Which keys of a tile a row sees, as bits, 32 a word.  words(): the part of the row's mask that the tile needs, N + 1 loads in
 // flight at once, which may be made ahead; bits(): the tile's keys from j0 on.
@@ -258,11 +286,11 @@ template <int ROWS, int KEYS>
 __device__ __forceinline__ void leave_unit(const Args& a, const Walk<ROWS, KEYS>& w, const Piece& p) {
   if (!p.begins || p.ends) return;
   const int to = w.at + (p.x.first_tile + p.x.tiles - p.tile_hi), r0 = p.block * ROWS;
-  a.part_units[blockIdx.x] = make_int4(w.share_of(to - 1) - blockIdx.x + 1, r0, p.x.q0,
-                                       p.kvh | min(ROWS, p.x.q_len * (a.nq / a.nkv) - r0) << 16);
+  a.part_units[blockIdx.x] = make_int4((w.share_of(to - 1) - blockIdx.x / w.members + 1) | w.members << 16, r0, p.x.q0,
+                                       p.kvh | min(ROWS, p.x.q_len * a.g - r0) << 16);
 }
 
-// Adds the slabs of the unit that begins in share blockIdx.x and goes on behind it: out = sum_z O_z 2^(m_z - M) / sum_z l_z
+// Adds the slabs of the unit that begins in block blockIdx.x's share and goes on behind it: out = sum_z O_z 2^(m_z - M) / sum_z l_z
 // 2^(m_z - M), M the largest reference of a slab that saw a key; which slabs a warp adds depends on their number alone.
 // A block has 32 rows (blockIdx.y), a lane one of them and MERGE_DIMS dimensions (of units of 16 rows a warp has two such runs);
 // what warps the dimensions leave deal the slabs among themselves and add up in shared memory.  The kernel is all latency -- the
@@ -281,14 +309,14 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) tree_merge_kernel(const __gr
   pdl_wait();
   pdl_trigger();
   const int4 unit = a.part_units[share];
-  const int slabs = unit.x, kvh = unit.w & 0xffff, rows = unit.w >> 16;
+  const int slabs = unit.x & 0xffff, members = unit.x >> 16, kvh = unit.w & 0xffff, rows = unit.w >> 16;
   if (slabs == 0 || (int)blockIdx.y * RL >= rows) return;
   float acc[MERGE_DIMS], M = -CUDART_INF_F, L = 0.f;
 #pragma unroll
   for (int i = 0; i < MERGE_DIMS; ++i) acc[i] = 0.f;
 #pragma unroll 2
   for (int z = row < rows ? turn : slabs; z < slabs; z += turns) {
-    const size_t slab = slab_of(share + z, z == 0);
+    const size_t slab = slab_of(share + z * members, z == 0);
     const float2 v = *reinterpret_cast<const float2*>(a.part_ml + (slab * ROWS + row) * 2);
     const float* src = a.part_o + (slab * a.hd + d0) * ROWS + row;
     float o[MERGE_DIMS];
@@ -328,7 +356,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) tree_merge_kernel(const __gr
   }
   if (row >= rows || dims <= 0) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  const int g = a.nq / a.nkv, r = unit.y + row;
+  const int g = a.g, r = unit.y + row;
   T* dst = (T*)a.out + ((size_t)(unit.z + r / g) * a.nq + kvh * g + r % g) * a.hd + d0;
 #pragma unroll
   for (int i = 0; i < MERGE_DIMS; ++i) acc[i] *= inv;
@@ -349,7 +377,7 @@ template <typename T, int ROWS>
 inline void launch_merge(const Args& a, int blocks, cudaStream_t stream) {
   constexpr int RL = ROWS < 32 ? ROWS : 32, SPAN = 32 / RL * MERGE_DIMS;
   const int dim_warps = (a.hd + SPAN - 1) / SPAN, turns = std::min(MERGE_TURNS, MERGE_WARPS / dim_warps);
-  const int max_rows = std::min(a.max_q_len * (a.nq / a.nkv), ROWS);
+  const int max_rows = std::min(a.max_q_len * a.g, ROWS);
   launch_pdl(tree_merge_kernel<T, ROWS>, dim3(blocks, (max_rows + RL - 1) / RL), dim3(32 * dim_warps * turns), 0, stream, a, dim_warps, turns);
 }
 

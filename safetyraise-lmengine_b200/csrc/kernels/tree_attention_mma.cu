@@ -53,11 +53,11 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
   const bf16* vc = (const bf16*)a.v_cache;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, mi = lane >> 3;
   const int row_warp = warp / KEY_WARPS, key0 = (warp % KEY_WARPS) * WK;
-  const int g = a.nq / a.nkv;
+  const int g = a.g;
   pdl_wait();
   pdl_trigger();
   Walk<ROWS, M_KEYS> walk;
-  walk.init(a, blockIdx.x, gridDim.x, blockIdx.x == 0);
+  walk.init(a, blockIdx.x == 0);
   Piece w;
   if (threadIdx.x == 0) leave_no_unit(a);
   while (walk.next(a, w)) {

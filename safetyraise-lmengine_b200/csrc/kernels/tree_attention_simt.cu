@@ -32,11 +32,11 @@ __global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const __grid_const
   const T* kc = (const T*)a.k_cache;
   const T* vc = (const T*)a.v_cache;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = a.nq / a.nkv;
+  const int g = a.g;
   pdl_wait();
   pdl_trigger();
   Walk<S_ROWS, S_KEYS> walk;
-  walk.init(a, blockIdx.x, gridDim.x, blockIdx.x == 0);
+  walk.init(a, blockIdx.x == 0);
   Piece w;
   if (threadIdx.x == 0) leave_no_unit(a);
   while (walk.next(a, w)) {

@@ -105,11 +105,11 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   pdl_wait();
   pdl_trigger();
 
-  const int g = a.nq / a.nkv;
+  const int g = a.g;
   using Walks = Walk<T_ROWS, T_KEYS>;
   Walks walk;
   if (warp <= 2 || warp == 10) {
-    walk.init(a, blockIdx.x, gridDim.x, blockIdx.x == 0 && warp == 0);
+    walk.init(a, blockIdx.x == 0 && warp == 0);
     if (warp == 2 && lane == 0) walk_sh = walk;    // (the softmax warps keep theirs in shared memory: its numbers would cost them registers)
   }
 
@@ -120,6 +120,8 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     uint8_t* ring = keys ? k_t : v_t;
     uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
     const int ps = a.page_size, box_rows = ps < T_KEYS ? ps : T_KEYS, boxes = T_KEYS / box_rows;
+    const int shift = 31 - __clz(ps);
+    const bool pages = ps & (ps - 1);              // of no power of two
     int k = 0;                                     // tiles so far
     bool ok = true;
     Piece w;
@@ -129,7 +131,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       // the lane's page of a tile, looked up a tile ahead (behind the entry's last key: page 0, which nobody sees)
       auto page_of = [&](int t) {
         const int key = t * T_KEYS + lane * box_rows;
-        return lane < boxes && t < w.tile_hi && key < w.x.kv_len ? table[key / ps] : 0;
+        return lane < boxes && t < w.tile_hi && key < w.x.kv_len ? table[pages ? key / ps : key >> shift] : 0;
       };
       int page_next = page_of(w.tile_lo);
       for (int t = w.tile_lo; t < w.tile_hi; ++t, ++k) {
@@ -141,7 +143,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           if (key + box_rows > first) atomicExch(a.err_flag, ERR_PAGE);      // (pages behind a window are given back)
           page = 0;
         }
-        const int row = (page * a.nkv + w.kvh) * ps + key % ps;
+        const int row = (page * a.nkv + w.kvh) * ps + (pages ? key % ps : key & (ps - 1));
         ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((k / STAGES) & 1) ^ 1, a.err_flag, 81));
         if (!ok) break;
         if (lane == 0) mbar_expect_tx(&full[s], TILE);
@@ -343,18 +345,12 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       if (ok && live) {
         // both streams' sums of the row, half of the columns each
         const bool two = tiles > 1;
-        float2 s0, s1 = make_float2(0.f, 0.f);
-        {
-          uint32_t ml[16];
-          tmem_ld16(tmem + lane_addr, ml);
-          tmem_wait_ld();
-          s0 = make_float2(__uint_as_float(ml[0]), __uint_as_float(ml[1]));
-          if (two) {
-            tmem_ld16(tmem + 128 + lane_addr, ml);
-            tmem_wait_ld();
-            s1 = make_float2(__uint_as_float(ml[0]), __uint_as_float(ml[1]));
-          }
-        }
+        uint32_t ml0[16], ml1[16];
+        tmem_ld16(tmem + lane_addr, ml0);
+        tmem_ld16(tmem + 128 + lane_addr, ml1);
+        tmem_wait_ld();
+        const float2 s0 = make_float2(__uint_as_float(ml0[0]), __uint_as_float(ml0[1]));
+        const float2 s1 = make_float2(__uint_as_float(ml1[0]), __uint_as_float(ml1[1]));
         const float M = two ? fmaxf(s0.x, s1.x) : s0.x, mb = M == -CUDART_INF_F ? 0.f : M;
         const float f0 = ex2(s0.x - mb), f1 = two ? ex2(s1.x - mb) : 0.f;
         const float L = two ? f0 * s0.y + f1 * s1.y : f0 * s0.y;
@@ -376,13 +372,6 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             o[j] = f0 * __uint_as_float(u[j]);
             if (two) o[j] = fmaf(f1, __uint_as_float(v[j]), o[j]);
           }
-          if (loose_sh && mine)
-#pragma unroll 1
-            for (int j = 0; j < 16; ++j) {
-              const float more = loose_values<T_KEYS>(a, x.start, x.kv_len, a.block_table + (size_t)w.e * a.table_stride, w.kvh, token, c + j, w.tile_lo, w.tile_hi);
-#pragma unroll
-              for (int n = 0; n < 16; ++n) o[n] += n == j ? more : 0.f;
-            }
           if (mine && whole) {
 #pragma unroll
             for (int n = 0; n < 2; ++n)
@@ -394,6 +383,15 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             for (int n = 0; n < 16; ++n) a.part_o[(slab * HD + c + n) * T_ROWS + row] = o[n];
           }
         }
+        if (loose_sh && mine)                      // (what a row sees of them outweighs all the rest)
+#pragma unroll 1
+          for (int c = i * (HD / 2); c < (i + 1) * (HD / 2); ++c) {
+            const float v = loose_values<T_KEYS>(a, x.start, x.kv_len, a.block_table + (size_t)w.e * a.table_stride, w.kvh, token, c, w.tile_lo, w.tile_hi);
+            if (!isfinite(v)) {
+              if (whole) dst[c] = from_float<bf16>(v);
+              else a.part_o[(slab * HD + c) * T_ROWS + row] = v;
+            }
+          }
         fence_before();
       }
       meet();                                      // O, S and the rows are free

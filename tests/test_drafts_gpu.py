@@ -165,6 +165,17 @@ def test_trees(lens, ctx, nq, nkv, hd, ps, dt, window):
     c.check()
 
 
+@pytest.mark.parametrize("dt, lens, ctx, nq, nkv, hd, ps", [
+    (torch.bfloat16, [64, 50], [9000, 12000], 64, 8, 128, 16),     # blocks of rows side by side over more keys than L2 holds
+    (torch.bfloat16, [64, 33, 50], [12000, 9000, 1], 16, 8, 256, 32),
+    (torch.bfloat16, [64, 5, 64], [9000, 4000, 9000], 40, 8, 128, 64),     # ... and entries of too unlike numbers of them
+    (torch.float32, [20, 20], [5000, 4500], 32, 8, 128, 16)])
+def test_long_contexts(dt, lens, ctx, nq, nkv, hd, ps):
+    c = Case(lens, ctx, nq, nkv, hd, ps, dt, seed=6)
+    c.run()
+    c.check()
+
+
 @pytest.mark.parametrize("dt, hd", [(torch.float32, 18), (torch.float32, 5), (torch.bfloat16, 36)])
 def test_heads_of_odd_sizes(dt, hd):
     c = Case([9, 14], [50, 120], 4, 2, hd, 16, dt, seed=hd)
