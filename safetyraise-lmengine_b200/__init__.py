@@ -36,7 +36,7 @@ __version__ = "0.1.0"
 
 
 def __getattr__(name):
-    if name in ("Engine", "StepEntry"):
+    if name in ("Engine", "StepEntry", "Verified"):
         from .engine import step
         return getattr(step, name)
     if name in ("LLM", "GenerationRequest", "EngineConfig"):

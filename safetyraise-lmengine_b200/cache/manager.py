@@ -94,6 +94,9 @@ def runtime():
         lib.srlm_cache_lay_out_pages.argtypes = [C.c_void_p, C.c_int, C.c_int, at, at, at, C.c_int, C.c_int, at, at]
         lib.srlm_sampling_uniforms.argtypes = [C.c_int, at, at, at]
         lib.srlm_sampling_uniforms.restype = None
+        for name, numbers in (("fork", 2), ("unshare", 2), ("compact", 0)):
+            fn = getattr(lib, "srlm_cache_" + name)
+            fn.restype, fn.argtypes = C.c_int, [C.c_void_p] + [C.c_int] * numbers + [at, C.c_int, C.POINTER(C.c_int)]
         lib.srlm_cache_destroy.argtypes = [C.c_void_p]
         lib.srlm_cache_reuse_counts.argtypes = [C.c_void_p, C.POINTER(C.c_int64), C.POINTER(C.c_int64)]
         lib.srlm_sched_destroy.argtypes = [C.c_void_p]
@@ -197,9 +200,66 @@ class CacheManager:
             raise ValueError(f"commit(slot={slot}, new_len={new_len}) is invalid ({r})")
 
     def truncate(self, slot: int, length: int) -> None:
+        """Forgets the slot's tokens from ``length`` on.  Where that is inside a page that another request holds too, the slot
+        gets a copy of the page first (ResourceExhausted without a free one, and nothing has changed)."""
         r = self._lib.srlm_cache_truncate(self._h, slot, length)
+        if r == -4:
+            if self._with_copies("unshare", len(self._paged), slot, length) == 0:
+                raise ResourceExhausted(f"no free page for the one that slot {slot} shares at token {length}")
+            r = self._lib.srlm_cache_truncate(self._h, slot, length)
         if r != 0:
             raise ValueError(f"truncate(slot={slot}, len={length}) is invalid ({r})")
+
+    # ---- pages in several requests' tables ----------------------------------------
+    def _with_copies(self, what: str, room: int, *args) -> int:
+        """Runs a native call that names pages to copy and copies them, in every pool of their groups, on the current stream."""
+        copies, n = np.empty((max(room, 1), 3), dtype=np.int32), C.c_int()
+        r = getattr(self._lib, "srlm_cache_" + what)(self._h, *args, copies.ctypes.data, max(room, 1), C.byref(n))
+        if r < 0:
+            return r
+        copies = copies[:n.value]
+        if self.device is not None and len(copies):
+            from ..kernels import ops
+            with torch.cuda.device(self.device):
+                for g, spec in enumerate(self._paged):
+                    mine = copies[copies[:, 0] == g]
+                    for pools in (self.kv_pools, self.k_pools, self.v_pools):
+                        if len(mine) and spec.name in pools:
+                            ops.copy_pages(pools[spec.name], mine[:, 1], mine[:, 2])
+        return r
+
+    def fork(self, slot: int, length: Optional[int] = None) -> int:
+        """A new request that begins with the first ``length`` tokens (default: all committed ones) of the one in ``slot``;
+        returns its slot.  The pages that those tokens fill are shared -- neither request writes them again --, the one
+        they end in is copied, and so is the fixed-size state, which only knows the request as it stands: with state
+        groups ``length`` is the request's own.  The copies run on the current stream, behind the steps launched on it; a step
+        of the request that may still be taken back is settled first."""
+        have = self.length(slot)
+        length = have if length is None else length
+        if self.state_groups and length != have:
+            raise ValueError(f"fork(slot={slot}, length={length}): the fixed-size state stands at {have} tokens")
+        r = self._with_copies("fork", len(self._paged), slot, length)
+        if r == -4:
+            raise ResourceExhausted(f"all {self.max_requests} request slots are taken")
+        if r == -5:
+            raise ResourceExhausted(f"no free page for the one that slot {slot} ends in at token {length}")
+        if r < 0:
+            raise ValueError(f"fork(slot={slot}, length={length}) is invalid ({r})")
+        for pool in self.state_pools.values():
+            pool[:, r].copy_(pool[:, slot])
+        return r
+
+    def compact(self) -> int:
+        """Moves the pages in use to the lowest numbers of every group's pool, contents and tables; returns how many moved.
+        Between steps only: a step that is laid out holds the old numbers."""
+        r = self._with_copies("compact", len(self._paged) * self.num_pages)
+        if r < 0:
+            raise ResourceExhausted("no memory to compact the pages")
+        return r
+
+    @property
+    def state_groups(self) -> List[CacheGroupSpec]:
+        return [g for g in self.groups if g.kind == FIXED_STATE]
 
     def length(self, slot: int) -> int:
         return self._lib.srlm_cache_length(self._h, slot)

@@ -14,11 +14,26 @@ CacheManager::CacheManager(int max_requests, const std::vector<GroupSpec>& group
     // page 0 is handed out first
     for (int p = s.num_pages - 1; p >= 0; --p) g.free_list.push_back(p);
     g.ever_used.assign(s.num_pages, 0);
+    g.holders.assign(s.num_pages, 0);
     groups_.push_back(std::move(g));
   }
   slots_.resize(max_requests);
   for (int s = max_requests - 1; s >= 0; --s) free_slots_.push_back(s);
   for (Slot& s : slots_) s.tables.resize(groups_.size());
+}
+
+int32_t CacheManager::take(Group& g) {
+  int32_t page = g.free_list.back();
+  g.free_list.pop_back();
+  pages_taken_ += 1;
+  if (g.ever_used[page]) pages_reused_ += 1;
+  g.ever_used[page] = 1;
+  g.holders[page] = 1;
+  return page;
+}
+
+void CacheManager::give(Group& g, int32_t page) {
+  if (--g.holders[page] == 0) g.free_list.push_back(page);
 }
 
 int CacheManager::open_request() {
@@ -39,7 +54,7 @@ int CacheManager::close_request(int slot) {
   Slot& s = slots_[slot];
   for (size_t g = 0; g < groups_.size(); ++g) {
     for (int32_t page : s.tables[g])
-      if (page >= 0) groups_[g].free_list.push_back(page);
+      if (page >= 0) give(groups_[g], page);
     s.tables[g].clear();
   }
   s.open = false;
@@ -71,14 +86,7 @@ int CacheManager::reserve(int slot, int new_len) {
   for (size_t g = 0; g < groups_.size(); ++g) {
     Group& grp = groups_[g];
     int want = ceil_div(new_len, grp.spec.page_size);
-    while (static_cast<int>(s.tables[g].size()) < want) {
-      int32_t page = grp.free_list.back();
-      grp.free_list.pop_back();
-      pages_taken_ += 1;
-      if (grp.ever_used[page]) pages_reused_ += 1;
-      grp.ever_used[page] = 1;
-      s.tables[g].push_back(page);
-    }
+    while (static_cast<int>(s.tables[g].size()) < want) s.tables[g].push_back(take(grp));
   }
   s.reserved = std::max(s.reserved, new_len);
   return 1;
@@ -107,7 +115,7 @@ int CacheManager::commit(int slot, int new_len) {
     int first = std::min(first_needed_page(grp, new_len), static_cast<int>(s.tables[g].size()));
     for (int p = kept_pages(grp); p < first; ++p) {
       if (s.tables[g][p] >= 0) {
-        grp.free_list.push_back(s.tables[g][p]);
+        give(grp, s.tables[g][p]);
         s.tables[g][p] = -1;
       }
     }
@@ -129,17 +137,105 @@ int CacheManager::truncate(int slot, int len) {
     }
   }
   for (size_t g = 0; g < groups_.size(); ++g) {
+    const int at = len / groups_[g].spec.page_size;
+    if (len % groups_[g].spec.page_size && at < static_cast<int>(s.tables[g].size()) && s.tables[g][at] >= 0 &&
+        groups_[g].holders[s.tables[g][at]] > 1) return -4;
+  }
+  for (size_t g = 0; g < groups_.size(); ++g) {
     Group& grp = groups_[g];
     int keep = ceil_div(len, grp.spec.page_size);
     while (static_cast<int>(s.tables[g].size()) > keep) {
       int32_t page = s.tables[g].back();
       s.tables[g].pop_back();
-      if (page >= 0) grp.free_list.push_back(page);
+      if (page >= 0) give(grp, page);
     }
   }
   s.length = std::min(s.length, len);
   s.reserved = len;
   return 0;
+}
+
+int CacheManager::fork(int slot, int len, std::vector<PageCopy>* copies) {
+  if (!valid(slot) || len < 0) return -1;
+  if (len > slots_[slot].length) return -2;
+  for (size_t g = 0; g < groups_.size(); ++g) {
+    const Group& grp = groups_[g];
+    const auto& t = slots_[slot].tables[g];
+    const int pages = ceil_div(len, grp.spec.page_size);
+    for (int p = std::max(first_needed_page(grp, len), kept_pages(grp)); p < pages; ++p)
+      if (t[p] < 0) return -3;
+    if (len % grp.spec.page_size && grp.free_list.empty()) return -5;
+  }
+  const int made = open_request();
+  if (made < 0) return -4;
+  const Slot& from = slots_[slot];
+  Slot& to = slots_[made];
+  for (size_t g = 0; g < groups_.size(); ++g) to.tables[g].reserve(ceil_div(len, groups_[g].spec.page_size));
+  for (size_t g = 0; g < groups_.size(); ++g) {
+    Group& grp = groups_[g];
+    const int full = len / grp.spec.page_size;
+    for (int p = 0; p < full; ++p) {
+      const int32_t page = from.tables[g][p];
+      if (page >= 0) grp.holders[page] += 1;
+      to.tables[g].push_back(page);
+    }
+    if (len % grp.spec.page_size) {
+      const int32_t page = take(grp);
+      copies->push_back(PageCopy{static_cast<int32_t>(g), from.tables[g][full], page});
+      to.tables[g].push_back(page);
+    }
+  }
+  to.length = to.reserved = len;
+  return made;
+}
+
+int CacheManager::unshare(int slot, int len, std::vector<PageCopy>* copies) {
+  if (!valid(slot) || len < 0 || len > slots_[slot].reserved) return -1;
+  Slot& s = slots_[slot];
+  auto shared = [&](size_t g) {
+    const int at = len / groups_[g].spec.page_size;
+    return len % groups_[g].spec.page_size && at < static_cast<int>(s.tables[g].size()) && s.tables[g][at] >= 0 &&
+           groups_[g].holders[s.tables[g][at]] > 1;
+  };
+  for (size_t g = 0; g < groups_.size(); ++g)
+    if (shared(g) && groups_[g].free_list.empty()) return 0;
+  for (size_t g = 0; g < groups_.size(); ++g) {
+    if (!shared(g)) continue;
+    int32_t& mine = s.tables[g][len / groups_[g].spec.page_size];
+    const int32_t page = take(groups_[g]);
+    copies->push_back(PageCopy{static_cast<int32_t>(g), mine, page});
+    give(groups_[g], mine);
+    mine = page;
+  }
+  return 1;
+}
+
+int CacheManager::compact(std::vector<PageCopy>* copies) {
+  int moved = 0;
+  for (size_t g = 0; g < groups_.size(); ++g) {
+    Group& grp = groups_[g];
+    int used = 0;
+    for (int32_t h : grp.holders) used += h > 0;
+    std::vector<int32_t> now(grp.spec.num_pages);
+    int32_t hole = 0;
+    for (int32_t p = 0; p < grp.spec.num_pages; ++p) {
+      now[p] = p;
+      if (p < used || grp.holders[p] == 0) continue;
+      while (grp.holders[hole] > 0) ++hole;            // below `used`: as many holes there as pages in use beyond
+      now[p] = hole;
+      grp.holders[hole] = grp.holders[p];
+      grp.holders[p] = 0;
+      grp.ever_used[hole] = 1;
+      copies->push_back(PageCopy{static_cast<int32_t>(g), p, hole});
+      ++moved;
+    }
+    for (Slot& s : slots_)
+      for (int32_t& p : s.tables[g])
+        if (p >= 0) p = now[p];
+    grp.free_list.clear();
+    for (int32_t p = grp.spec.num_pages - 1; p >= used; --p) grp.free_list.push_back(p);
+  }
+  return moved;
 }
 
 int CacheManager::length(int slot) const { return valid(slot) ? slots_[slot].length : -1; }
@@ -173,25 +269,30 @@ int CacheManager::peak_pages(int group, int total_len, int max_step) const {
 int CacheManager::audit() const {
   for (size_t g = 0; g < groups_.size(); ++g) {
     const Group& grp = groups_[g];
-    std::vector<int> seen(grp.spec.num_pages, 0);
+    std::vector<int> seen(grp.spec.num_pages, 0), freed(grp.spec.num_pages, 0);
     for (int32_t p : grp.free_list) {
       if (p < 0 || p >= grp.spec.num_pages) return 1;   // id out of range
-      seen[p] += 1;
+      freed[p] += 1;
     }
     for (const Slot& s : slots_) {
       if (!s.open) {
         if (!s.tables[g].empty()) return 2;             // closed slot still holds pages
         continue;
       }
+      std::vector<int32_t> own;
       for (int32_t p : s.tables[g]) {
         if (p < 0) continue;
         if (p >= grp.spec.num_pages) return 1;
         seen[p] += 1;
+        own.push_back(p);
       }
+      std::sort(own.begin(), own.end());
+      if (std::adjacent_find(own.begin(), own.end()) != own.end()) return 4;      // twice in one table
     }
-    for (int c : seen) {
-      if (c == 0) return 3;                             // page lost
-      if (c > 1) return 4;                              // page held or freed twice
+    for (int p = 0; p < grp.spec.num_pages; ++p) {
+      if (seen[p] + freed[p] == 0) return 3;            // page lost
+      if (freed[p] > 1 || (freed[p] && seen[p])) return 4;   // freed twice, or held and free
+      if (seen[p] != grp.holders[p]) return 6;          // miscounted
     }
   }
   std::vector<int> slot_seen(slots_.size(), 0);

@@ -7,6 +7,11 @@
 // in which case pages that the window has passed are given back at commit.
 // Each group has pages of its own.  A request holds one slot; the slot index
 // also addresses the request's fixed-size state in every state group.
+// A page may stand in several requests' tables (a fork shares the pages that
+// are full up to where it begins); it is free again when the last one lets go.
+// No page that more than one table holds is ever written: a request only writes
+// behind its length, and where its length ends inside a page that page is its own
+// (fork and unshare name the copies that make it so; the caller carries them out).
 //
 // Counterpart of PagedKvCache / SequenceState in the reference
 // (src/engine/state.rs:19-224), which keeps pages per request on the heap;
@@ -29,6 +34,10 @@ struct GroupSpec {
   int keep_first = 0;  // first tokens of a sequence that stay visible behind the window: their pages are never given back early
 };
 
+struct PageCopy {
+  int32_t group, src, dst;
+};
+
 class CacheManager {
  public:
   CacheManager(int max_requests, const std::vector<GroupSpec>& groups);
@@ -44,8 +53,19 @@ class CacheManager {
   int commit(int slot, int new_len);
   // Forgets tokens from len on and gives back pages no longer needed (ALL groups only
   // shrink; a window group cannot bring back released pages, so len must not go below
-  // what its window still covers: returns <0 then).
+  // what its window still covers: returns <0 then).  -4: len ends inside a page that another
+  // request holds too; unshare() first.
   int truncate(int slot, int len);
+  // A new request that begins with the first len tokens of slot's: its slot, with the pages that len fills shared
+  // and a copy of the one that it ends in (added to *copies).  -1 slot not open, -2 len is beyond its length, -3 a window
+  // has passed pages that len needs, -4 no slot free, -5 no page free (nothing changed in either case).
+  int fork(int slot, int len, std::vector<PageCopy>* copies);
+  // Makes the page that len ends in the slot's own in every group, by a copy (added to *copies) where another request
+  // holds it too: 1 done, 0 not enough free pages (nothing changed), <0 bad arguments.
+  int unshare(int slot, int len, std::vector<PageCopy>* copies);
+  // Puts the pages in use together at the lowest numbers, in every group: tables as after the copies that are added to
+  // *copies (none reads a page that another writes).  The number of pages moved.
+  int compact(std::vector<PageCopy>* copies);
 
   int length(int slot) const;
   int reserved_tokens(int slot) const;
@@ -60,7 +80,7 @@ class CacheManager {
   int peak_pages(int group, int total_len, int max_step) const;
   int64_t pages_taken_total() const { return pages_taken_; }
   int64_t pages_reused_total() const { return pages_reused_; }
-  // 0 when every page of every group is either free once or held by exactly one table once.
+  // 0 when every page of every group is either free once or held by as many tables as its count says.
   int audit() const;
 
  private:
@@ -68,6 +88,7 @@ class CacheManager {
     GroupSpec spec;
     std::vector<int32_t> free_list;        // LIFO: the page freed last is used next
     std::vector<uint8_t> ever_used;
+    std::vector<int32_t> holders;          // tables that a page stands in
   };
   struct Slot {
     bool open = false;
@@ -78,6 +99,8 @@ class CacheManager {
   };
   int first_needed_page(const Group& g, int length) const;
   int kept_pages(const Group& g) const;     // leading pages that hold tokens every later query sees
+  int32_t take(Group& g);                   // a free page, held once now
+  void give(Group& g, int32_t page);        // one holder less
   bool valid(int slot) const { return slot >= 0 && slot < max_requests() && slots_[slot].open; }
 
   std::vector<Group> groups_;

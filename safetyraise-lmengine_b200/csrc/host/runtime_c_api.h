@@ -17,6 +17,12 @@ int srlm_cache_reserve(void* cache, int slot, int new_len);
 int srlm_cache_fit_tokens(void* cache, int slot, int want_len);
 int srlm_cache_commit(void* cache, int slot, int new_len);
 int srlm_cache_truncate(void* cache, int slot, int len);
+/* Pages in several tables.  copies: 3 words each (group, source page, destination page), at most `room` of them; the number is
+ * written to *n.  fork: the new slot, or <0; unshare: 1, 0 without free pages, <0; compact: pages moved.  <0 as beside the methods;
+ * -9: no memory, or no room for the copies (nothing changed). */
+int srlm_cache_fork(void* cache, int slot, int len, int32_t* copies, int room, int* n);
+int srlm_cache_unshare(void* cache, int slot, int len, int32_t* copies, int room, int* n);
+int srlm_cache_compact(void* cache, int32_t* copies, int room, int* n);
 int srlm_cache_length(void* cache, int slot);
 int srlm_cache_reserved(void* cache, int slot);
 int srlm_cache_generation(void* cache, int slot);

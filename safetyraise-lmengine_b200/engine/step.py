@@ -22,7 +22,7 @@ import torch
 
 from ..cache.manager import CacheManager
 from ..config.registry import architecture_of, read_config_json
-from ..errors import ConfigError, ResourceExhausted, ShapeError, StepFailed, Unavailable
+from ..errors import ConfigError, ResourceExhausted, ShapeError, StepFailed, Unavailable, Unsupported
 from ..parts.base import (FAULT_LOGITS, FAULT_NAMES, FAULT_TOKEN, STATUS_WORDS, ModelContext, StepContext,
                           Workspace)
 from ..weights.safetensors_io import WeightFolder
@@ -41,6 +41,15 @@ class StepEntry:
     want: Sequence[int] = ()          # indices into ``tokens`` whose logits are returned
     generation: Optional[int] = None  # the slot's generation when the request opened it (``Engine.generation``);
                                       # given, a step refuses a slot that another request holds by now
+    parents: Optional[Sequence[int]] = None   # ``Engine.verify``: each token's parent among ``tokens``, -1 for the first;
+                                      # None: every token follows the one before it
+
+
+@dataclass
+class Verified:
+    """What ``Engine.verify`` kept of an entry."""
+    path: List[int]                   # places among the entry's tokens, from the first on down the tree
+    next_token: int                   # the model's own choice behind the last of them
 
 
 @dataclass
@@ -61,6 +70,7 @@ class PreparedStep:
     state_snapshot: Optional[dict] = None   # fixed-size state of the step's slots before the forward
     host: Optional[np.ndarray] = None       # the pinned buffer as an array (made once: set_token is called per token)
     arrays: Optional[tuple] = None          # (slots, lengths behind the step) as int32 arrays
+    drafts: bool = False                    # tokens of trees (Engine.verify)
 
     def set_token(self, entry: int, index: int, token: int) -> None:
         h = self.host if self.host is not None else self.pair[0].numpy()
@@ -146,6 +156,17 @@ class Engine:
     def close_request(self, slot: int) -> None:
         self.cache.close_request(slot)
 
+    def fork_request(self, slot: int, length: Optional[int] = None) -> int:
+        """A new request that begins with the first ``length`` tokens (default: all) of the one in ``slot``: the pages they
+        fill are shared, the one they end in and the fixed-size state are copied (CacheManager.fork).  Returns its slot."""
+        with torch.cuda.device(self.mctx.device):
+            if self.cache.state_pools and slot < len(self._slot_generation) \
+                    and self._slot_generation[slot] != self.cache.generation(slot):
+                raise ShapeError(f"slot {slot} has run no step yet: its fixed-size state is another request's")
+            made = self.cache.fork(slot, length)
+        self._slot_generation[made] = self.cache.generation(made)      # its state is set: not to be zeroed at its first step
+        return made
+
     # ---- the step -------------------------------------------------------------
     def _validate(self, entries: Sequence[StepEntry]):
         """Checks the entries; -> (slots as an int32 array, lengths, generations) of their slots."""
@@ -202,7 +223,8 @@ class Engine:
             pair[1].synchronize()
         return pair, self._meta_dev
 
-    def _lay_out(self, entries: Sequence[StepEntry], starts: List[int], slots: Optional[np.ndarray] = None) -> PreparedStep:
+    def _lay_out(self, entries: Sequence[StepEntry], starts: List[int], slots: Optional[np.ndarray] = None,
+                 drafts: bool = False) -> PreparedStep:
         """Flattens the batch into a pinned host buffer (no device work)."""
         n = len(entries)
         q_lens = [len(e.tokens) for e in entries]
@@ -224,6 +246,8 @@ class Engine:
             place(name, T)
         for g in groups:
             place("kv_slot:" + g.name, T)
+        if drafts:
+            place("parents", T)
         place("slots", n)
         place("cu_q", n + 1)
         place("kv_lens", n)
@@ -266,9 +290,12 @@ class Engine:
                 t0 += q
         if R:
             view("logit_rows")[:] = rows
+        if drafts:
+            view("parents")[:] = np.concatenate([np.arange(-1, len(e.tokens) - 1) if e.parents is None else np.asarray(e.parents)
+                                                 for e in entries])
         return PreparedStep(entries=entries, starts=starts, q_lens=q_lens, kv_lens=kv_lens, sections=sections,
                             words=off, pair=pair, pages=pages, wanted=R, token_at=token_at, missing=missing, host=h,
-                            arrays=(slots, starts_a + q_a))
+                            arrays=(slots, starts_a + q_a), drafts=drafts)
 
     def _upload(self, prep: PreparedStep) -> StepContext:
         """Copies the laid-out batch to the device in one copy and returns the device views."""
@@ -298,7 +325,7 @@ class Engine:
                   "slots": [e.slot for e in prep.entries]},
             cache=self.cache, workspace=self.workspace, dtype=self.mctx.dtype,
             max_q_len=max(prep.q_lens), max_kv_len=max(prep.kv_lens), kv_bound=pages * self.cache.page_size,
-            options=self.mctx.options, status=self.status[:STATUS_WORDS])
+            options=self.mctx.options, status=self.status[:STATUS_WORDS], parents=d("parents") if prep.drafts else None)
 
     def build_context(self, entries: Sequence[StepEntry], starts: List[int]) -> StepContext:
         """Flattens the batch, uploads it in one copy and returns the device views."""
@@ -307,7 +334,7 @@ class Engine:
     def _recorded(self, prep: PreparedStep) -> Optional[torch.Tensor]:
         """Replays the CUDA graph of this kind of step, if there is one (its kernels read the batch from where it was sent:
         no views are needed); else None."""
-        if not self.use_graphs or max(prep.q_lens) != 1 or self._graph_generation != self.workspace.generation:
+        if not self.use_graphs or prep.drafts or max(prep.q_lens) != 1 or self._graph_generation != self.workspace.generation:
             return None
         hit = self._graphs.get((len(prep.entries), len(prep.entries), prep.wanted, prep.pages * self.cache.page_size))
         return self._replay(hit) if hit is not None else None
@@ -323,7 +350,9 @@ class Engine:
     def _forward(self, ctx: StepContext) -> torch.Tensor:
         """Runs the model on the batch: eagerly, or by replaying the CUDA graph of this kind of step."""
         from ..kernels import ops
-        if not self.use_graphs or ctx.max_q_len != 1:
+        if ctx.parents is not None:
+            ctx.draft_mask()                          # also the tokens' positions, which everything below reads
+        if not self.use_graphs or ctx.max_q_len != 1 or ctx.parents is not None:
             return self.model.forward(ctx)
         if self._graph_generation != self.workspace.generation:   # a buffer moved since recording
             self._graphs.clear()
@@ -345,10 +374,12 @@ class Engine:
             ops.launches = before
         return self._replay(hit)
 
-    def prepare(self, entries: Sequence[StepEntry]) -> PreparedStep:
+    def prepare(self, entries: Sequence[StepEntry], drafts: bool = False) -> PreparedStep:
         """The host half of a step: checks, page reservation, batch layout.  Token ids given as LATER
         may be supplied afterwards (``PreparedStep.set_token``).  Between prepare() and run() or
-        discard() of a step no other step may be prepared or run."""
+        discard() of a step no other step may be prepared or run.  drafts: of ``verify``."""
+        if not drafts and any(e.parents is not None for e in entries):
+            raise ShapeError("entries with parents are drafted tokens: Engine.verify runs them")
         slots, starts, generations = self._validate(entries)
         self._greet_new_occupants(entries, generations)
         starts_a = np.array(starts, dtype=np.int32)
@@ -359,7 +390,7 @@ class Engine:
                                     f"({s}+{len(e.tokens)} tokens); nothing was run")
         try:
             with torch.cuda.device(self.mctx.device):
-                return self._lay_out(entries, starts, slots)
+                return self._lay_out(entries, starts, slots, drafts)
         except Exception:
             self.discard_reservation(entries, starts)
             raise
@@ -487,3 +518,58 @@ class Engine:
             raise fault
         self.commit(prep)
         return logits
+
+    # ---- drafted tokens -----------------------------------------------------------
+    def _check_drafts(self, entries: Sequence[StepEntry]) -> None:
+        blocks = getattr(self.model, "blocks", ())
+        if self.cache.state_pools or not blocks or not all(getattr(getattr(b, "mixer", None), "takes_drafts", False) for b in blocks):
+            raise Unsupported("drafted tokens need mixers that know their requests from paged keys alone (paged attention)")
+        for e in entries:
+            n = len(e.tokens)
+            if e.want:
+                raise ShapeError("verify() returns tokens, no logits: an entry of it wants none")
+            if any(int(t) == LATER for t in e.tokens):
+                raise ShapeError("drafted tokens are given, none is left open")
+            if e.parents is not None:
+                p = [int(x) for x in e.parents]
+                if len(p) != n or (n and p[0] != -1) or any(not 0 <= x < i for i, x in enumerate(p) if i):
+                    raise ShapeError(f"parents of {n} tokens are -1 for the first and an earlier token's place for each other")
+
+    def verify(self, entries: Sequence[StepEntry]) -> List[Verified]:
+        """Runs each entry's drafted tokens in one step and keeps those that the model itself would have chosen.
+
+        An entry's first token is the request's next one, the others were drafted behind it: ``parents`` names each
+        one's parent (None: a chain).  Every token sees the request's committed tokens and those it descends from.  The
+        walk from the first token goes to the first child whose token is the model's greedy choice behind the one before;
+        the tokens on it are committed, their keys and values side by side, and the rest is forgotten.  Each entry
+        gets at least its first token and one token more (``next_token``, not run yet).  A step that fails keeps nothing
+        (StepFailed), as in ``step``."""
+        self._check_drafts(entries)
+        prep = self.prepare([StepEntry(e.slot, e.tokens, range(len(e.tokens)), e.generation, e.parents) for e in entries], drafts=True)
+        logits = self.launch(prep)
+        n, room, T = len(entries), max(prep.q_lens), sum(prep.q_lens)
+        with torch.cuda.device(self.mctx.device):
+            from ..kernels import ops
+            ctx = self._context(prep)
+            targets = self.workspace.get("drafts.targets", T, 1, torch.int32).view(T)
+            ops.argmax(logits, targets, self.status[FAULT_LOGITS:FAULT_LOGITS + 1])
+            kept = self.workspace.get("drafts.kept", n, room + 2, torch.int32).view(-1)[:n * (room + 2)]
+            path, count, following = kept[2 * n:].view(n, room), kept[:n], kept[n:2 * n]
+            ops.accept_drafts(ctx.token_ids, ctx.parents, targets, ctx.cu_q, path, count, following)
+            for g in self.cache.paged_groups:
+                for pools in (self.cache.kv_pools, self.cache.k_pools, self.cache.v_pools):
+                    if g.name in pools:
+                        ops.keep_drafts(pools[g.name], ctx.block_tables[g.name], ctx.cu_q, ctx.kv_lens, path, count)
+            found = kept.tolist()
+        fault = self.fault_of(self.read_faults())
+        if fault is not None:
+            self.revoke(prep)
+            raise fault
+        result = []
+        for e, (entry, start) in enumerate(zip(prep.entries, prep.starts)):
+            self.cache.commit(entry.slot, start + found[e])
+            self.cache.truncate(entry.slot, start + found[e])
+            line = found[2 * n + e * room:2 * n + (e + 1) * room]
+            result.append(Verified(line[:found[e]], found[n + e]))
+        self.steps_run += 1
+        return result

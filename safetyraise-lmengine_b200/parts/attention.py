@@ -22,6 +22,8 @@ from .linear import Linear
 
 @register_mixer("paged_attention")
 class PagedAttention(Part):
+    takes_drafts = True          # steps of drafted tokens (Engine.verify): rotation by position, keys by mask
+
     def __init__(self, spec: AttentionSpec, prefix: str, tensors: dict, mctx):
         if spec.bias:
             raise Unsupported("attention with bias is not implemented")
@@ -82,7 +84,7 @@ class PagedAttention(Part):
         # how the encoding turns q and k is the encoding's to say (pairing, rotary fraction): the kernels take it
         rot = self.position.rotation(ctx) if self.position is not None else None
         attended = ctx.workspace.get("attn.out", T, s.heads * s.head_dim, ctx.dtype)
-        if ops.attention_from_projection(ctx, qkv, k_pool, v_pool, attended, ctx.block_tables[group], self.q_norm_w,
+        if ctx.parents is None and ops.attention_from_projection(ctx, qkv, k_pool, v_pool, attended, ctx.block_tables[group], self.q_norm_w,
                                          self.k_norm_w, self.eps, rot, run_step.writes_cache, s.heads,
                                          s.kv_heads, s.head_dim, k_pool.shape[2], s.softmax_scale, s.window or 0):
             return attended
@@ -91,6 +93,11 @@ class PagedAttention(Part):
                                 rot.cos if rot else None, rot.sin if rot else None, ctx.kv_slot[group], s.heads,
                                 s.kv_heads, s.head_dim, rot.pairs if rot else 0, write_kv=run_step.writes_cache,
                                 interleaved=bool(rot and rot.interleaved))
+        if ctx.parents is not None:
+            ops.tree_attention(q, k_pool, v_pool, attended, ctx.block_tables[group], ctx.cu_q, ctx.kv_lens,
+                               ctx.draft_mask(s.window or 0), s.heads, s.kv_heads, s.head_dim, k_pool.shape[2], s.softmax_scale,
+                               ctx.max_q_len, positions=ctx.positions, window=s.window or 0)
+            return attended
         ops.paged_attention(ctx, q, k_pool, v_pool, attended, ctx.block_tables[group], s.heads, s.kv_heads,
                             s.head_dim, k_pool.shape[2], s.softmax_scale, s.window or 0)
         return attended

@@ -146,6 +146,17 @@ class StepContext:
     kv_bound: int = 1                         # an upper bound of max_kv_len that kernels may size their grids by
     options: dict = field(default_factory=dict)   # the engine's options, for parts that have switches
     status: Optional[torch.Tensor] = None     # int32 [STATUS_WORDS]: the step's fault words (None: the model's own)
+    parents: Optional[torch.Tensor] = None    # int32 [T]: the tokens are drafted ones, each entry's a tree (ops.draft_tree)
+
+    def draft_mask(self, window: int = 0) -> torch.Tensor:
+        """int32 [T, words]: which of its entry's tokens each drafted token sees under a window; made once a step."""
+        key = ("draft_mask", window)
+        if key not in self.tables:
+            from ..kernels import ops
+            mask = self.workspace.get(f"drafts.mask{window}", self.T, -(-self.max_q_len // 32), torch.int32)
+            ops.draft_tree(self.parents, self.cu_q, self.kv_lens, self.positions, mask, window)
+            self.tables[key] = mask
+        return self.tables[key]
 
 
 @dataclass
