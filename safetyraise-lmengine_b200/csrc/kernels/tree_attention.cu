@@ -11,7 +11,7 @@ static Kind kind_of(int dtype, int hd, int page_size) {
   return tree::tcgen05_takes(hd, page_size) ? TCGEN05 : MMA;
 }
 static tree::Form form_of(Kind kind, int hd, int max_rows, int sms) {
-  return kind == TCGEN05 ? tree::tcgen05_form(sms) : kind == MMA ? tree::mma_form(hd, max_rows, sms) : tree::simt_form(hd, sms);
+  return kind == TCGEN05 ? tree::tcgen05_form(sms) : kind == MMA ? tree::mma_form(hd, max_rows, sms) : tree::simt_form(hd, max_rows, sms);
 }
 
 // float32 words of workspace that srlm_tree_attention wants for these sizes, or -1 where it refuses them.
@@ -58,6 +58,6 @@ extern "C" int srlm_tree_attention(const void* q, const void* k_cache, const voi
     a.least_tiles = 2;
     return kind == TCGEN05 ? tree::run_tcgen05(a, sms, stream) : tree::run_mma(a, max_rows, sms, stream);
   }
-  a.least_tiles = 4;
-  return tree::run_simt(a, dtype, sms, stream);
+  a.least_tiles = 2;
+  return tree::run_simt(a, dtype, max_rows, sms, stream);
 }

@@ -337,7 +337,7 @@ __device__ __forceinline__ void leave_unit(const Args& a, const Walk<ROWS, KEYS>
 
 // Adds the slabs of the unit that begins in block blockIdx.x's share and goes on behind it: out = sum_z O_z 2^(m_z - M) / sum_z l_z
 // 2^(m_z - M), M the largest reference of a slab that saw a key; which slabs a warp adds depends on their number alone.
-// A block has 32 rows (blockIdx.y), a lane one of them and MERGE_DIMS dimensions (of units of 16 rows a warp has two such runs);
+// A block has 32 rows (blockIdx.y), a lane one of them and MERGE_DIMS dimensions (of units of fewer rows a warp has several such runs);
 // what warps the dimensions leave deal the slabs among themselves and add up in shared memory.  The kernel is all latency -- the
 // unit's record, the slabs, the result -- and the code of one round is what it fetches: written out for several slabs at once, or with
 // a pass of its own for the references, it took 10 us and more where this takes 3.
@@ -442,8 +442,8 @@ inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<int> (&
 struct Form {
   int blocks, rows, keys;
 };
-Form simt_form(int hd, int sms);
-int run_simt(const Args& a, int dtype, int sms, cudaStream_t stream);
+Form simt_form(int hd, int max_rows, int sms);
+int run_simt(const Args& a, int dtype, int max_rows, int sms, cudaStream_t stream);
 bool mma_takes(int hd);                            // bfloat16
 Form mma_form(int hd, int max_rows, int sms);
 int run_mma(const Args& a, int max_rows, int sms, cudaStream_t stream);

@@ -159,16 +159,7 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
           }
         }
       }
-      float mx[2] = {-CUDART_INF_F, -CUDART_INF_F};
-      if (plain) {
-#pragma unroll
-        for (int nt = 0; nt < NS; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            s[nt][i] *= a.scale_log2;
-            mx[i >> 1] = fmaxf(mx[i >> 1], s[nt][i]);
-          }
-      } else {
+      if (!plain) {
         constexpr int NW = (WK + 31) / 32;
         uint32_t bits[2][NW];
 #pragma unroll
@@ -178,16 +169,20 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int k = nt * 8 + (lane & 3) * 2 + (i & 1);
-            s[nt][i] = (bits[i >> 1][(nt * 8) / 32] >> (k & 31)) & 1 ? s[nt][i] * a.scale_log2 : -CUDART_INF_F;
-            mx[i >> 1] = fmaxf(mx[i >> 1], s[nt][i]);
+            if (!((bits[i >> 1][(nt * 8) / 32] >> (k & 31)) & 1)) s[nt][i] = -CUDART_INF_F;      // (the score scale is positive)
           }
       }
+      float mx[2] = {-CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+      for (int nt = 0; nt < NS; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[i >> 1] = fmaxf(mx[i >> 1], s[nt][i]);
       float base[2], sum[2] = {0.f, 0.f}, alpha[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-        mx[i] = fmaxf(mx[i], m[i]);
+        mx[i] = fmaxf(mx[i] * a.scale_log2, m[i]);
         base[i] = mx[i] == -CUDART_INF_F ? 0.f : mx[i];
         alpha[i] = ex2(m[i] - base[i]);
         m[i] = mx[i];
@@ -197,7 +192,7 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
       for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t p = pack_bf16(ex2(s[nt][2 * i] - base[i]), ex2(s[nt][2 * i + 1] - base[i]));
+          const uint32_t p = pack_bf16(ex2(fmaf(s[nt][2 * i], a.scale_log2, -base[i])), ex2(fmaf(s[nt][2 * i + 1], a.scale_log2, -base[i])));
           sum[i] += __uint_as_float(p << 16) + __uint_as_float(p & 0xffff0000u);
           pf[nt >> 1][(nt & 1) * 2 + i] = p;
         }
@@ -234,21 +229,18 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
     __syncthreads();                                             // the tiles' memory is free
     const bool loose = loose_sh != 0, whole = w.begins && w.ends;
     const size_t slab = slab_of(blockIdx.x, w.begins);
-    // two neighbouring numbers of a row, sums with reference mr and total lr
-    auto put = [&](int row, int d, float v0, float v1, float inv) {
-      if (loose) {
-        const int t = x.q0 + (r0 + row) / g;
-        v0 += loose_values<M_KEYS>(a, x.start, x.kv_len, table, w.kvh, t, d, w.tile_lo, w.tile_hi);
-        v1 += loose_values<M_KEYS>(a, x.start, x.kv_len, table, w.kvh, t, d + 1, w.tile_lo, w.tile_hi);
-      }
+    auto out_of = [&](int row) {
+      const int r = r0 + row;
+      return (bf16*)a.out + ((size_t)(x.q0 + r / g) * a.nq + w.kvh * g + r % g) * hd;
+    };
+    // two neighbouring numbers of a row
+    auto put = [&](int row, bf16* dst, int d, float v0, float v1, float inv) {
       if (whole) {
-        const int r = r0 + row;
-        bf16* dst = (bf16*)a.out + ((size_t)(x.q0 + r / g) * a.nq + w.kvh * g + r % g) * hd + d;
-        *reinterpret_cast<uint32_t*>(dst) = pack_bf16(v0 * inv, v1 * inv);
+        *reinterpret_cast<uint32_t*>(dst + d) = pack_bf16(v0 * inv, v1 * inv);
       } else {
-        float* dst = a.part_o + (slab * hd + d) * ROWS + row;
-        dst[0] = v0;
-        dst[ROWS] = v1;
+        float* part = a.part_o + (slab * hd + d) * ROWS + row;
+        part[0] = v0;
+        part[ROWS] = v1;
       }
     };
     if constexpr (KEY_WARPS == 1) {
@@ -257,10 +249,11 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
         const int row = ra + 8 * i;
         if (row >= rows) continue;
         const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+        bf16* dst = out_of(row);
         if (!whole && (lane & 3) == 0) *reinterpret_cast<float2*>(a.part_ml + (slab * ROWS + row) * 2) = make_float2(m[i], l[i]);
 #pragma unroll
         for (int dn = 0; dn < NO; ++dn)
-          if (dn * 8 < hd) put(row, dn * 8 + (lane & 3) * 2, o[dn][2 * i], o[dn][2 * i + 1], inv);
+          if (dn * 8 < hd) put(row, dst, dn * 8 + (lane & 3) * 2, o[dn][2 * i], o[dn][2 * i + 1], inv);
       }
     } else {
       float* o_sh = reinterpret_cast<float*>(kv_sh);             // [4 warps][16][hd]
@@ -294,10 +287,20 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
           v1 += f * v.y;
         }
         if (!whole && d == 0) *reinterpret_cast<float2*>(a.part_ml + (slab * ROWS + row) * 2) = make_float2(M, L);
-        put(row, d, v0, v1, L == 0.f ? 0.f : 1.f / L);
+        put(row, out_of(row), d, v0, v1, L == 0.f ? 0.f : 1.f / L);
       }
     }
     __syncthreads();                                             // before the next piece's rows and tiles
+    if (loose) {                                                 // (what a row sees of them outweighs all the rest)
+      for (int i = tid; i < rows * hd; i += M_THREADS) {
+        const int row = i / hd, d = i - row * hd;
+        const float v = loose_values<M_KEYS>(a, x.start, x.kv_len, table, w.kvh, x.q0 + (r0 + row) / g, d, w.tile_lo, w.tile_hi);
+        if (isfinite(v)) continue;
+        if (whole) out_of(row)[d] = from_float<bf16>(v);
+        else a.part_o[(slab * hd + d) * ROWS + row] = v;
+      }
+      __syncthreads();
+    }
   }
 }
 
