@@ -70,7 +70,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   uint64_t* o_done = p_ready + 2;                  // [2]
   uint64_t* q_full = o_done + 2;
   __shared__ Walk<T_ROWS, T_KEYS> walk_sh;
-  __shared__ Piece piece_sh;
+  __shared__ Piece piece_sh[2];
   __shared__ int more_sh;
   __shared__ uint32_t tmem_sh;
   __shared__ int loose_sh, failed_sh;
@@ -230,13 +230,13 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     uint32_t done = 0;                             // tiles of this stream so far
     int k = 0;                                     // tiles of the block so far
     bool ok = true;
-    const Piece& w = piece_sh;
-    const Entry& x = w.x;
-    for (;;) {
-      if (threadIdx.x == 64) more_sh = walk_sh.next(a, piece_sh);      // (the last piece's readers have met)
-      meet();
-      if (!more_sh) break;
+    if (threadIdx.x == 64) more_sh = walk_sh.next(a, piece_sh[0]);
+    meet();
+    for (int n = 0; more_sh; n ^= 1) {
+      const Piece& w = piece_sh[n];
+      const Entry& x = w.x;
       const int rows_total = x.q_len * g, r0 = w.block * T_ROWS, rows = min(T_ROWS, rows_total - r0), tiles = w.tile_hi - w.tile_lo;
+      const int first = a.window > 0 ? max(0, x.start - a.window + 1) : 0;
       // the rows -> shared memory, swizzled (zeros behind the last), eight loads of a thread in flight; the products that read the last
       // piece's are done (their tiles were waited for)
       const bf16* q = (const bf16*)a.q;
@@ -285,16 +285,20 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           ok = __all_sync(0xffffffffu, mbar_wait(&v_full[s], ((k + t) / STAGES) & 1, a.err_flag, 88));
           if (!ok) break;
           uint8_t* vt = v_t + s * TILE;
-          const int first = a.window > 0 ? max(0, x.start - a.window + 1) - j0 : 0, behind = x.kv_len - j0;
+          const int behind = x.kv_len - j0, edge = a.window > 0 ? x.kv_len - a.window - j0 : 0;      // some row does not see keys in front of the edge
+          const int from = edge > 0 ? 0 : max(x.start - j0, 0);
           bool loose = false;
-#pragma unroll 4
-          for (int n = 0; n < T_KEYS * CHUNKS / 128; ++n) {
-            const int idx = n * 128 + row, key = idx / CHUNKS;
+#pragma unroll 1
+          for (int idx = from * CHUNKS + row; idx < T_KEYS * CHUNKS; idx += 128) {
+            const int key = idx / CHUNKS;
             uint4* at = reinterpret_cast<uint4*>(vt + tile_addr(0, key, idx % CHUNKS));
-            uint4 v = *at;
-            const bool there = key >= first && key < behind, change = take_loose(v);
-            loose |= there && change;
-            if (!there || change) *at = there ? v : make_uint4(0, 0, 0, 0);
+            uint4 v = make_uint4(0, 0, 0, 0);
+            bool change = true;
+            if (key < behind && j0 + key >= first) {
+              v = *at;
+              loose |= change = take_loose(v);
+            }
+            if (change) *at = v;
           }
           if (loose) loose_sh = 1;
           fence_async_smem();
@@ -338,6 +342,8 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         tmem_st16(s_addr, ml);
         tmem_wait_st();
       }
+      Piece* following = &piece_sh[n ^ 1];
+      const int more = threadIdx.x == 64 ? walk_sh.next(a, *following) : 0;      // (while the other stream ends)
       fence_before();
       meet();
       fence_after();
@@ -361,26 +367,25 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         bf16* dst = (bf16*)a.out + ((size_t)token * a.nq + w.kvh * g + r % g) * HD;
         const uint32_t both = tmem + 256 + lane_addr;
 #pragma unroll 1
-        for (int c = i * (HD / 2); c < (i + 1) * (HD / 2); c += 16) {
-          uint32_t u[16], v[16];
-          tmem_ld16(both + c, u);
-          if (two) tmem_ld16(both + 128 + c, v);
+        for (int c = i * (HD / 2); c < (i + 1) * (HD / 2); c += 32) {
+          uint32_t u[32], v[32];
+          tmem_ld32(both + c, u);
+          tmem_ld32(both + 128 + c, v);
           tmem_wait_ld();
-          float o[16];
+          float o[32];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
+          for (int j = 0; j < 32; ++j) {
             o[j] = f0 * __uint_as_float(u[j]);
             if (two) o[j] = fmaf(f1, __uint_as_float(v[j]), o[j]);
           }
           if (mine && whole) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
-              *reinterpret_cast<uint4*>(dst + c + 8 * n) =
-                  make_uint4(pack2(o[8 * n] * inv, o[8 * n + 1] * inv), pack2(o[8 * n + 2] * inv, o[8 * n + 3] * inv),
-                             pack2(o[8 * n + 4] * inv, o[8 * n + 5] * inv), pack2(o[8 * n + 6] * inv, o[8 * n + 7] * inv));
+            for (int n8 = 0; n8 < 32; n8 += 8)
+              *reinterpret_cast<uint4*>(dst + c + n8) = make_uint4(pack2(o[n8] * inv, o[n8 + 1] * inv), pack2(o[n8 + 2] * inv, o[n8 + 3] * inv),
+                                                                   pack2(o[n8 + 4] * inv, o[n8 + 5] * inv), pack2(o[n8 + 6] * inv, o[n8 + 7] * inv));
           } else if (mine) {
 #pragma unroll
-            for (int n = 0; n < 16; ++n) a.part_o[(slab * HD + c + n) * T_ROWS + row] = o[n];
+            for (int j = 0; j < 32; ++j) a.part_o[(slab * HD + c + j) * T_ROWS + row] = o[j];
           }
         }
         if (loose_sh && mine)                      // (what a row sees of them outweighs all the rest)
@@ -394,6 +399,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           }
         fence_before();
       }
+      if (threadIdx.x == 64) more_sh = more;
       meet();                                      // O, S and the rows are free
       if (st == 0) loose_sh = 0;                   // (read before the meeting, set behind the next piece's first tile)
       if (!ok) break;
