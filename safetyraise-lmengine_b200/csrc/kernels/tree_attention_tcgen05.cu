@@ -31,7 +31,7 @@ template <int HD>
 struct TmaForm {
   static constexpr int TILE = T_KEYS * HD * 2;     // bytes of a tile of keys, values or rows
   static constexpr int STAGES = HD == 128 ? 3 : 6;
-  static constexpr int SMEM = TILE * (1 + 2 * STAGES) + 1024 + (4 * STAGES + 7) * 8;
+  static constexpr int SMEM = TILE * (1 + 2 * STAGES) + 1024 + (4 * STAGES + 9) * 8;
 };
 
 __device__ __forceinline__ bool elected() {
@@ -51,6 +51,52 @@ __device__ __forceinline__ void mask_row(Row& r, const uint32_t (&bits)[4]) {
   part(r.d, bits[3]);
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float row_top(const Row& r) {
+  float m[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+  auto part = [&](const uint32_t (&v)[32]) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) m[(j >> 1) & 3] = max3(m[(j >> 1) & 3], __uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+  };
+  part(r.a);
+  part(r.b);
+  part(r.c);
+  part(r.d);
+  return max3(fmaxf(m[0], m[1]), m[2], m[3]);
+}
+// The weights exp2(S * scale - base) of 64 keys as bfloat16 pairs over columns of S; their sum, pairs by pairs.
+__device__ __forceinline__ float2 half_exp(uint32_t addr, const uint32_t (&va)[32], const uint32_t (&vb)[32], float scale, float base) {
+  const float2 sc = make_float2(scale, scale), nb = make_float2(-base, -base);
+  float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+  auto part = [&](const uint32_t (&v)[32], uint32_t at) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      float2 x = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), sc, nb);
+      float2 y = fma2(make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), sc, nb);
+      x = make_float2(ex2(x.x), ex2(x.y));
+      y = make_float2(ex2(y.x), ex2(y.y));
+      pk[j >> 1] = pack2(x.x, x.y);
+      pk[(j >> 1) + 1] = pack2(y.x, y.y);
+      s0 = add2(s0, x);
+      s1 = add2(s1, y);
+    }
+    tmem_st16(at, pk);
+  };
+  part(va, addr);
+  part(vb, addr + 16);
+  return add2(s0, s1);
+}
+
 template <int HD>
 __global__ void __launch_bounds__(T_THREADS, 1)
 tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a) {
@@ -67,7 +113,8 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   uint64_t* v_empty = v_full + STAGES;
   uint64_t* s_full = v_empty + STAGES;             // [2]: per stream
   uint64_t* p_ready = s_full + 2;                  // [2]
-  uint64_t* o_done = p_ready + 2;                  // [2]
+  uint64_t* p_half = p_ready + 2;                  // [2]: the weights of a tile's first 64 keys
+  uint64_t* o_done = p_half + 2;                   // [2]
   uint64_t* q_full = o_done + 2;
   __shared__ Walk<T_ROWS, T_KEYS> walk_sh;
   __shared__ Piece piece_sh[2];
@@ -86,6 +133,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_ready[i], 4);
+      mbar_init(&p_half[i], 4);
       mbar_init(&o_done[i], 1);
     }
     mbar_init(q_full, T_SOFTMAX / 32);
@@ -201,17 +249,25 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       if (tiles > 1) issue_s(1);
       for (int t = 0; t < tiles && ok; ++t) {
         const int i = t & 1;
+        const uint64_t vd = v_desc + (uint64_t)(s_v * (TILE >> 4));
+        const uint32_t d = tm + 256 + i * 128, p = tm + i * 128;
         ok = __all_sync(0xffffffffu, mbar_wait(&v_full[s_v], v_phase, a.err_flag, 85) &&
-                                         mbar_wait(&p_ready[i], (p_phase >> i) & 1, a.err_flag, 86));
+                                         mbar_wait(&p_half[i], (p_phase >> i) & 1, a.err_flag, 86));
+        if (!ok) break;
+        fence_after();
+        if (issues) {
+#pragma unroll
+          for (int kk = 0; kk < T_KEYS / 32; ++kk)   // 16 keys: 8 columns of pairs, 2048 bytes of values
+            umma_bf16_ts(d, p + kk * 8, vd + kk * (2048 >> 4), idesc_o, t > 1 || kk > 0);
+        }
+        __syncwarp();
+        ok = __all_sync(0xffffffffu, mbar_wait(&p_ready[i], (p_phase >> i) & 1, a.err_flag, 91));
         if (!ok) break;
         p_phase ^= 1u << i;
         fence_after();
-        const uint64_t vd = v_desc + (uint64_t)(s_v * (TILE >> 4));
-        const uint32_t d = tm + 256 + i * 128, p = tm + i * 128;
         if (issues) {
 #pragma unroll
-          for (int kk = 0; kk < T_KEYS / 16; ++kk)   // 16 keys: 8 columns of pairs, 2048 bytes of values
-            umma_bf16_ts(d, p + kk * 8, vd + kk * (2048 >> 4), idesc_o, t > 1 || kk > 0);
+          for (int kk = T_KEYS / 32; kk < T_KEYS / 16; ++kk) umma_bf16_ts(d, p + kk * 8, vd + kk * (2048 >> 4), idesc_o, 1);
           umma_commit(&o_done[i]);
           umma_commit(&v_empty[s_v]);
         }
@@ -307,7 +363,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           Row srow;
           load_row(s_addr, srow);
           if (!plain) mask_row(srow, bits);
-          const float mx = row_max<false>(srow, 0, T_KEYS) * a.scale_log2;
+          const float mx = row_top(srow) * a.scale_log2;
           const bool grow = mx > m_run + T_RESCALE_ABOVE || m_run == -CUDART_INF_F;
           const float m_new = grow ? fmaxf(mx, m_run) : m_run;
           if (any && __any_sync(0xffffffffu, m_new != m_run)) {
@@ -327,8 +383,16 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           }
           m_run = m_new;
           const float base = m_run == -CUDART_INF_F ? 0.f : m_run;
-          l_run += row_exp<false>(s_addr, srow, a.scale_log2, base, 0, T_KEYS);
+          const float2 s0 = half_exp(s_addr, srow.a, srow.b, a.scale_log2, base);
           tmem_wait_st();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_half[i]);
+          const float2 s1 = add2(s0, half_exp(s_addr + 32, srow.c, srow.d, a.scale_log2, base));
+          l_run += s1.x + s1.y;
+          tmem_wait_st();
+        } else if (lane == 0) {
+          mbar_arrive(&p_half[i]);
         }
         fence_before();
         __syncwarp();
