@@ -359,22 +359,30 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) tree_merge_kernel(const __gr
   float acc[MERGE_DIMS], M = -CUDART_INF_F, L = 0.f;
 #pragma unroll
   for (int i = 0; i < MERGE_DIMS; ++i) acc[i] = 0.f;
-#pragma unroll 2
-  for (int z = row < rows ? turn : slabs; z < slabs; z += turns) {
-    const size_t slab = slab_of(share + z * members, z == 0);
-    const float2 v = *reinterpret_cast<const float2*>(a.part_ml + (slab * ROWS + row) * 2);
-    const float* src = a.part_o + (slab * a.hd + d0) * ROWS + row;
-    float o[MERGE_DIMS];
+  constexpr int AHEAD = 2;                                           // slabs in flight (four: 2 us more, for their code)
+  for (int z0 = row < rows ? turn : slabs; z0 < slabs; z0 += AHEAD * turns) {
+    float2 v[AHEAD];
+    float o[AHEAD][MERGE_DIMS];
 #pragma unroll
-    for (int i = 0; i < MERGE_DIMS; ++i) o[i] = i < dims ? src[i * ROWS] : 0.f;
-    if (v.y > 0.f) {                                                 // (a slab of no key holds nothing)
-      const float m_new = fmaxf(M, v.x), f = exp2f(v.x - m_new), old = exp2f(M - m_new);
-      M = m_new;
-      L = L * old + f * v.y;
+    for (int k = 0; k < AHEAD; ++k) {
+      const int z = z0 + k * turns;
+      const size_t slab = slab_of(share + z * members, z == 0);
+      const float* src = a.part_o + (slab * a.hd + d0) * ROWS + row;
+      v[k] = z < slabs ? *reinterpret_cast<const float2*>(a.part_ml + (slab * ROWS + row) * 2) : make_float2(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < MERGE_DIMS; ++i) acc[i] = acc[i] * old + f * o[i];
-    } else if (v.y != v.y) {
-      L = v.y;                                                       // (a score that was no number makes the row none)
+      for (int i = 0; i < MERGE_DIMS; ++i) o[k][i] = z < slabs && i < dims ? src[i * ROWS] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      if (v[k].y > 0.f) {                                            // (a slab of no key holds nothing)
+        const float m_new = fmaxf(M, v[k].x), f = exp2f(v[k].x - m_new), old = exp2f(M - m_new);
+        M = m_new;
+        L = L * old + f * v[k].y;
+#pragma unroll
+        for (int i = 0; i < MERGE_DIMS; ++i) acc[i] = acc[i] * old + f * o[k][i];
+      } else if (v[k].y != v[k].y) {
+        L = v[k].y;                                                  // (a score that was no number makes the row none)
+      }
     }
   }
   if (turns > 1) {

@@ -9,8 +9,9 @@
 // warps form the weights of a tile, the tensor core works for the other, and three stages of keys and values (six of heads of
 // 64) are in flight.  At the end of a piece the two streams' sums are joined as they are read from tensor memory (a warp reads
 // the same lanes of both; each stream's warps write half of the columns).
-// Warps 0 and 10 fetch keys and values (a lane a page box), one thread of warp 1 issues the MMAs, warps 2-5 and 6-9 are the
-// streams' softmax.  A block
+// Warps 0, 10 and 11 fetch tiles of keys and of values in turn (a lane a page box; an issue takes 70 ns beside busy softmax warps, and a
+// tile of pages of 16 has 16 boxes), one thread of warp 1 issues the MMAs, warps 2-5 and 6-9 are the streams' softmax.  The softmax
+// bounds calls of many rows: 1.45 us a tile and stream, of which 0.55 are its exponentials alone, beside 0.9 us of products.  A block
 // stays for all of its pieces: the fetches run ahead across them, and the block count is the SMs'.
 //
 // A weight is rounded to bfloat16 for the product with the values.  O is rescaled only when a row's maximum has grown by more
@@ -24,7 +25,7 @@ namespace tree {
 
 using namespace fmha;
 
-constexpr int T_ROWS = 128, T_KEYS = 128, T_THREADS = 352, T_SOFTMAX = 256;
+constexpr int T_ROWS = 128, T_KEYS = 128, T_THREADS = 384, T_SOFTMAX = 256, T_PRODUCERS = 3;
 constexpr float T_RESCALE_ABOVE = 8.f;             // log2 of the growth of a row's maximum that O is rescaled for
 
 template <int HD>
@@ -156,21 +157,18 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   const int g = a.g;
   using Walks = Walk<T_ROWS, T_KEYS>;
   Walks walk;
-  if (warp <= 2 || warp == 10) {
+  if (warp <= 2 || warp >= 10) {
     walk.init(a, blockIdx.x == 0 && warp == 0);
     if (warp == 2 && lane == 0) walk_sh = walk;    // (the softmax warps keep theirs in shared memory: its numbers would cost them registers)
   }
 
-  if (warp == 0 || warp == 10) {
-    // ---------------- TMA producers: keys, values ----------------
-    const bool keys = warp == 0;
-    const CUtensorMap* map = keys ? &map_k : &map_v;
-    uint8_t* ring = keys ? k_t : v_t;
-    uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
-    const int ps = a.page_size, box_rows = ps < T_KEYS ? ps : T_KEYS, boxes = T_KEYS / box_rows;
+  const int ps = a.page_size, box_rows = ps < T_KEYS ? ps : T_KEYS;
+  if (warp == 0 || warp >= 10) {
+    // ---------------- TMA producers ----------------
+    const int producer = warp == 0 ? 0 : warp - 9, boxes = T_KEYS / box_rows;
     const int shift = 31 - __clz(ps);
     const bool pages = ps & (ps - 1);              // of no power of two
-    int k = 0;                                     // tiles so far
+    int job = 0, k = 0;                            // tiles of keys and of values in turn, so far; tiles of keys
     bool ok = true;
     Piece w;
     while (ok && walk.next(a, w)) {
@@ -182,7 +180,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         return lane < boxes && t < w.tile_hi && key < w.x.kv_len ? table[pages ? key / ps : key >> shift] : 0;
       };
       int page_next = page_of(w.tile_lo);
-      for (int t = w.tile_lo; t < w.tile_hi; ++t, ++k) {
+      for (int t = w.tile_lo; t < w.tile_hi && ok; ++t, ++k) {
         const int s = k % STAGES;
         int page = page_next;
         page_next = page_of(t + 1);
@@ -192,19 +190,26 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           page = 0;
         }
         const int row = (page * a.nkv + w.kvh) * ps + (pages ? key % ps : key & (ps - 1));
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((k / STAGES) & 1) ^ 1, a.err_flag, 81));
-        if (!ok) break;
-        if (lane == 0) mbar_expect_tx(&full[s], TILE);
-        __syncwarp();
-        uint8_t* tile = ring + s * TILE + lane * box_rows * 128;
-        if (lane < boxes) {
+        for (int values = 0; values < 2; ++values, ++job) {
+          if (job % T_PRODUCERS != producer) continue;
+          uint64_t *full = values ? &v_full[s] : &k_full[s], *empty = values ? &v_empty[s] : &k_empty[s];
+          ok = __all_sync(0xffffffffu, mbar_wait(empty, ((k / STAGES) & 1) ^ 1, a.err_flag, 81));
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(full, TILE);
+          __syncwarp();
+          if (lane < boxes) {
+            uint8_t* tile = (values ? v_t : k_t) + s * TILE + lane * box_rows * 128;
 #pragma unroll
-          for (int c = 0; c < HD; c += 64) tma_load_2d(tile + c * (T_KEYS * 2), map, &full[s], c, row);
+            for (int c = 0; c < HD; c += 64) tma_load_2d(tile + c * (T_KEYS * 2), values ? &map_v : &map_k, full, c, row);
+          }
         }
       }
     }
     if (!ok)                                       // copies in flight end before the block does
-      for (int back = 1; back <= STAGES && back <= k; ++back) mbar_wait(&full[(k - back) % STAGES], ((k - back) / STAGES) & 1, a.err_flag, 82);
+      for (int back = 1; back <= STAGES && back <= k; ++back) {
+        mbar_wait(&k_full[(k - back) % STAGES], ((k - back) / STAGES) & 1, a.err_flag, 82);
+        mbar_wait(&v_full[(k - back) % STAGES], ((k - back) / STAGES) & 1, a.err_flag, 82);
+      }
     __syncwarp();
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
