@@ -18,9 +18,15 @@
 // Small work is divided along the units instead: each into as many equal parts as keep every block at one part.  A block whose
 // share reaches into a second unit begins anew with its rows and its first keys, which costs it SPARE_TILES tiles' time (8 entries of
 // 128 rows behind 2,000 keys, 8 KV heads: 33.8 us by shares of all tiles, 29.5 by parts of units).
+// Small work is divided along the units instead: each into as many equal parts as keep every block at one part.  A block whose
+// share reaches into a second unit begins anew with its rows and its first keys and leaves two slabs, which costs it more than
+// SPARE_TILES tiles (entries of 128 rows, 8 KV heads of 128, us, shares of all tiles | parts: 1 behind 600 keys 22.1 | 15.8, 8
+// behind 2,000 29.9 | 25.8, 16 behind 2,000 51.5 | 34.7, 16 behind 4,000 68.1 | 56.0, 12 behind 8,000 77.0 | 82.5, which is beyond
+// the 12 spare tiles).
 // Where units of several blocks of rows read more keys than the L2 cache holds, their blocks go through the same tiles at the same
 // time, as many thread blocks side by side as the units have blocks of rows (members): the keys come from memory once and not once
-// for each (8 entries of 320 rows behind up to 32,768 keys: 380 us apart, 316 side by side).
+// for each (8 entries behind 12,000 to 24,000 keys, 8 KV heads of 128, us, apart | side by side: 320 rows 273 | 237; behind 8,000 to
+// 16,000, 512 rows 263 | 212, 256 rows 141 | 122; 256 rows behind 4,000, which the cache holds, 59.7 | 58.5).
 #pragma once
 
 #include <math_constants.h>
@@ -99,7 +105,7 @@ struct Piece {
   bool begins, ends;           // the unit's first tile, its last one, are the piece's
 };
 
-constexpr int SPARE_TILES = 4;
+constexpr int SPARE_TILES = 12;
 constexpr float L2_HELD = 64e6f;     // bytes of keys and values that units read one behind another still find in the L2 cache
 
 // A block's share of the list.  Every warp that calls next() walks the same pieces.  (A list is shorter than 2^31: the entry

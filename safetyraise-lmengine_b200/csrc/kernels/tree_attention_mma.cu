@@ -1,5 +1,5 @@
 // Attention for drafted tokens on bfloat16 tensor cores at warp level (mma.sync m16n8k16, float32 accumulation): heads of any
-// multiple of 16 up to 256, any page size, and the calls of few rows.  What a row sees and how the work is divided:
+// multiple of 16 up to 256, any page size.  What a row sees and how the work is divided:
 // tree_attention.cuh.
 //
 // A block's four warps share a tile of 64 keys, fetched with cp.async through the block table (the rows' addresses are found
@@ -305,7 +305,8 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
 }
 
 // ---------------------------------------------------------------------------
-// Warps along the keys: by the rows that an entry has at most.
+// Warps along the keys: by the rows that an entry has at most (8 KV heads of 128, pages of 20, 8 entries behind 8,000 keys, us, four |
+// two | one: 16 rows 60.7 | 63.0 | 68.9, 32 rows 104 | 65.5 | 77.6, 64 rows 183 | 114 | 83.2).
 static int key_warps(int max_rows) { return max_rows <= 16 ? 4 : max_rows <= 32 ? 2 : 1; }
 static int blocks_per_sm(int hd) { return hd <= 64 ? 3 : hd <= 128 ? 2 : 1; }
 
