@@ -172,16 +172,18 @@ __global__ void __launch_bounds__(KEEP_THREADS) keep_drafts_kernel(V* __restrict
 }
 
 // ---------------------------------------------------------------------------
-// Pages: slab by slab, page dst[i] takes what page src[i] holds.  The numbers travel in the launch.
+// Pages: slab by slab, page dst[i] takes what page src[i] holds.
 // ---------------------------------------------------------------------------
-constexpr int COPY_THREADS = 256, COPY_PAIRS = 480, COPY_AHEAD = 8;
+// The numbers travel in the launch: 480 pairs, or 16, which spare a small call the copy of 4 KB of parameters.
+constexpr int COPY_THREADS = 256, COPY_AHEAD = 8, COPY_MANY = 480, COPY_FEW = 16;
+template <int PAIRS>
 struct Pairs {
-  int src[COPY_PAIRS], dst[COPY_PAIRS];
+  int src[PAIRS], dst[PAIRS];
 };
 
 // block: COPY_THREADS * each pieces of a page; x runs over a page's chunks, y over pairs and slabs
-template <typename V>
-__global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(V* __restrict__ pool, const __grid_constant__ Pairs pairs, int n,
+template <typename V, int PAIRS>
+__global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(V* __restrict__ pool, const __grid_constant__ Pairs<PAIRS> pairs, int n,
                                                                   long long slab_pages, long long page_pieces, int chunks) {
   pdl_wait();
   pdl_trigger();
@@ -217,6 +219,32 @@ static int with_pieces(int bytes, F f) {
     case 4: return f((uint32_t)0);
     default: return f((uint16_t)0);
   }
+}
+
+template <int PAIRS>
+static int copy_in(void* pool, long long slabs, long long num_pages, long long page_bytes, const long long* src, const long long* dst, int n,
+                   int sms, cudaStream_t stream) {
+  const int bytes = piece_bytes(pool, page_bytes);
+  const long long pieces = page_bytes / bytes;
+  for (int i0 = 0; i0 < n; i0 += PAIRS) {
+    Pairs<PAIRS> p;
+    const int here = std::min(PAIRS, n - i0);
+    for (int i = 0; i < here; ++i) p.src[i] = (int)src[i0 + i], p.dst[i] = (int)dst[i0 + i];
+    // a thread's eight pieces in flight, unless that leaves SMs without a block
+    long long chunks = (pieces + COPY_THREADS * COPY_AHEAD - 1) / (COPY_THREADS * COPY_AHEAD);
+    const long long most = (pieces + COPY_THREADS - 1) / COPY_THREADS;
+    while (chunks < most && chunks * here * slabs < 4ll * sms) chunks = std::min(most, 2 * chunks);
+    const long long blocks = chunks * here * slabs;
+    if (blocks > 0x7fffffff) return refuse(ST_BAD_SIZE, "copy_pages: %lld blocks", blocks);
+    const int status = with_pieces(bytes, [&](auto v) {
+      using V = decltype(v);
+      launch_pdl(copy_pages_kernel<V, PAIRS>, dim3((unsigned)blocks), dim3(COPY_THREADS), 0, stream, (V*)pool, p, here, num_pages, pieces,
+                 (int)chunks);
+      return launched();
+    });
+    if (status != ST_OK) return status;
+  }
+  return ST_OK;
 }
 
 }  // namespace drafts
@@ -286,24 +314,6 @@ extern "C" int srlm_copy_pages(void* pool, long long slabs, long long num_pages,
   } catch (...) {
     return refuse(ST_BAD_SIZE, "copy_pages: no host memory for %d page numbers", n);
   }
-  const int bytes = piece_bytes(pool, page_bytes);
-  const long long pieces = page_bytes / bytes;
-  for (int i0 = 0; i0 < n; i0 += COPY_PAIRS) {
-    Pairs p;
-    const int here = std::min(COPY_PAIRS, n - i0);
-    for (int i = 0; i < here; ++i) p.src[i] = (int)src[i0 + i], p.dst[i] = (int)dst[i0 + i];
-    // a thread's eight pieces in flight, unless that leaves SMs without a block
-    long long chunks = (pieces + COPY_THREADS * COPY_AHEAD - 1) / (COPY_THREADS * COPY_AHEAD);
-    const long long most = (pieces + COPY_THREADS - 1) / COPY_THREADS;
-    while (chunks < most && chunks * here * slabs < 4ll * sms) chunks = std::min(most, 2 * chunks);
-    const long long blocks = chunks * here * slabs;
-    if (blocks > 0x7fffffff) return refuse(ST_BAD_SIZE, "copy_pages: %lld blocks", blocks);
-    const int status = with_pieces(bytes, [&](auto v) {
-      using V = decltype(v);
-      launch_pdl(copy_pages_kernel<V>, dim3((unsigned)blocks), dim3(COPY_THREADS), 0, stream, (V*)pool, p, here, num_pages, pieces, (int)chunks);
-      return launched();
-    });
-    if (status != ST_OK) return status;
-  }
-  return ST_OK;
+  return n <= COPY_FEW ? copy_in<COPY_FEW>(pool, slabs, num_pages, page_bytes, src, dst, n, sms, stream)
+                       : copy_in<COPY_MANY>(pool, slabs, num_pages, page_bytes, src, dst, n, sms, stream);
 }

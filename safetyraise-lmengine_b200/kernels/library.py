@@ -999,19 +999,29 @@ class KernelLibrary:
         is written twice, and none is both read and written."""
         what, here = "copy_pages", self._here()
         at, slabs, pages, page = self._page_pool(what, pool, here)
-        numbers = []
-        for x in (src, dst):
-            if isinstance(x, torch.Tensor) and x.is_cuda:
-                raise ShapeError("copy_pages: page numbers are the host's")
-            x = np.asarray(x)
-            if x.ndim != 1 or (x.size and x.dtype.kind not in "iu"):
-                raise ShapeError(f"copy_pages: page numbers are a list of whole numbers, got {x.dtype} {list(x.shape)}")
-            numbers.append(np.ascontiguousarray(x, dtype=np.int64))
-        if numbers[0].size != numbers[1].size:
-            raise ShapeError(f"copy_pages: {numbers[0].size} pages to {numbers[1].size}")
-        self._check(self._entry("srlm_copy_pages")(
-            at, slabs, pages, page[0] * page[1] * page[2] * pool.element_size(), numbers[0].ctypes.data, numbers[1].ctypes.data,
-            numbers[0].size, self.sm_count(pool.device), self._raw_stream(here)), what)
+        n = len(src)
+        if n != len(dst):
+            raise ShapeError(f"copy_pages: {n} pages to {len(dst)}")
+        numbers = [self._page_numbers(x, n, pages) for x in (src, dst)]
+        self._check(self._entry("srlm_copy_pages")(at, slabs, pages, page[0] * page[1] * page[2] * pool.element_size(), numbers[0],
+                                                   numbers[1], n, self.sm_count(pool.device), self._raw_stream(here)), what)
+
+    @staticmethod
+    def _page_numbers(x, n, pages):
+        """Page numbers of the host as a C array (kept alive by the caller through the call); the native side checks them."""
+        if type(x) is list:
+            try:
+                if n and not 0 <= min(x) <= max(x) < pages:        # (a C number would lose the upper bits of a larger one)
+                    raise ShapeError(f"copy_pages: page {min(x) if min(x) < 0 else max(x)} is outside the pool of {pages}")
+                return (C.c_longlong * n)(*x)
+            except TypeError:            # numbers of another type than Python's own
+                pass
+        if isinstance(x, torch.Tensor) and x.is_cuda:
+            raise ShapeError("copy_pages: page numbers are the host's")
+        x = np.asarray(x)
+        if x.ndim != 1 or (x.size and x.dtype.kind not in "iu"):
+            raise ShapeError(f"copy_pages: page numbers are a list of whole numbers, got {x.dtype} {list(x.shape)}")
+        return (C.c_longlong * n).from_buffer_copy(np.ascontiguousarray(x, dtype=np.int64)) if n else (C.c_longlong * 1)()
 
     # ---- blocks that norm on both sides of a sublayer --------------------------------
     def gated_postnorm_add(self, residual, sub, gate, gate_bias, post_w, eps, next_w=None, next_eps=0.0,

@@ -588,7 +588,7 @@ def test_refusals():
     with pytest.raises(ShapeError):
         ops.accept_drafts(ints([1, 2]), ints([-1]), ints([1, 2]), ints([0, 2]), ints([[0]]), ints([0]), ints([0]))
     pool = torch.zeros(2, 6, 1, 4, 8, device=DEV)
-    for src, dst in (([0], [6]), ([-1], [0]), ([0, 1], [2, 2]), ([0, 1], [1, 2]), ([3], [3]), ([0], [1, 2]), ([0.5], [1]), ([[0]], [[1]]),
+    for src, dst in (([0], [6]), ([-1], [0]), ([2 ** 64], [1]), (np.array([7]), [1]), ([0], np.array([-1])), ([0, 1], [2, 2]), ([0, 1], [1, 2]), ([3], [3]), ([0], [1, 2]), ([0.5], [1]), ([[0]], [[1]]),
                      (ints([0]), [1])):
         with pytest.raises(ShapeError):
             ops.copy_pages(pool, src, dst)
