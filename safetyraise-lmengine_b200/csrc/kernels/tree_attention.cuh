@@ -23,6 +23,9 @@
 // SPARE_TILES tiles (entries of 128 rows, 8 KV heads of 128, us, shares of all tiles | parts: 1 behind 600 keys 22.1 | 15.8, 8
 // behind 2,000 29.9 | 25.8, 16 behind 2,000 51.5 | 34.7, 16 behind 4,000 68.1 | 56.0, 12 behind 8,000 77.0 | 82.5, which is beyond
 // the 12 spare tiles).
+// More units than blocks are dealt out whole where that is no longer, a beginning and the merge counted as BEGIN_TILES tiles each
+// (entries of 64 rows, us, shares of all tiles | whole units: 32 behind 600 keys 41.5 | 30.6, 64 behind 1,000 75.4 | 68.0; 20 behind
+// 2,000, two rounds of 17 tiles, 47.9 | 55.8).
 // Where units of several blocks of rows read more keys than the L2 cache holds, their blocks go through the same tiles at the same
 // time, as many thread blocks side by side as the units have blocks of rows (members): the keys come from memory once and not once
 // for each (8 entries behind 12,000 to 24,000 keys, 8 KV heads of 128, us, apart | side by side: 320 rows 273 | 237; behind 8,000 to
@@ -105,7 +108,7 @@ struct Piece {
   bool begins, ends;           // the unit's first tile, its last one, are the piece's
 };
 
-constexpr int SPARE_TILES = 12;
+constexpr int SPARE_TILES = 12, BEGIN_TILES = 10;
 constexpr float L2_HELD = 64e6f;     // bytes of keys and values that units read one behind another still find in the L2 cache
 
 // A block's share of the list.  Every warp that calls next() walks the same pieces.  (A list is shorter than 2^31: the entry
@@ -113,13 +116,16 @@ constexpr float L2_HELD = 64e6f;     // bytes of keys and values that units read
 template <int ROWS, int KEYS>
 struct Walk {
   int at, end;                 // the next tile and the share's end
-  int members, member;         // thread blocks side by side on a share, each with a block of rows; 1: shares of all units' tiles
+  int members, member;         // thread blocks side by side on a share, each with a block of rows; 1: shares of all units' tiles;
+                               // 0: of whole units, and what counts tiles here counts units
   int each, more;              // tiles of a share; the first `more` shares have one more
   int e, base;                 // entry of the tile `at`, whose list begins at `base`
   int parts;                   // 0, or of how many parts of its unit this block has one: `at` the unit, `base` the part
   Entry x;
 
-  __device__ __forceinline__ int weight(const Args& a, const Entry& y) const { return y.tiles * a.nkv * (members > 1 ? 1 : y.blocks); }
+  __device__ __forceinline__ int weight(const Args& a, const Entry& y) const {
+    return a.nkv * (members > 1 ? y.tiles : members == 1 ? y.tiles * y.blocks : y.blocks);
+  }
   __device__ __forceinline__ int first_of(int share) const { return share * each + min(share, more); }
   // the share that holds the tile `pos`
   __device__ __forceinline__ int share_of(int pos) const {
@@ -131,7 +137,8 @@ struct Walk {
   __device__ __forceinline__ void init(const Args& a, bool flag) {
     const int lane = threadIdx.x & 31, there = gridDim.x;
     Entry mine;
-    int whole = 0, single = 0, most = 0;         // tiles of all units, of one block of rows each; most blocks of rows
+    int whole = 0, single = 0, most = 0, units = 0, longest = 0;      // tiles of all units, of one block of rows each; most blocks of
+                                                 // rows; units, and most tiles of one
     for (int e0 = 0; e0 < a.n; e0 += 32) {
       if (e0 + lane < a.n) mine = entry_of<ROWS, KEYS>(a, e0 + lane, flag);
       else mine.tiles = mine.blocks = 0;
@@ -139,14 +146,16 @@ struct Walk {
       single += __reduce_add_sync(0xffffffffu, w);
       whole += __reduce_add_sync(0xffffffffu, w * mine.blocks);
       most = max(most, __reduce_max_sync(0xffffffffu, mine.blocks));
+      units += __reduce_add_sync(0xffffffffu, mine.blocks * a.nkv);
+      longest = max(longest, __reduce_max_sync(0xffffffffu, mine.tiles));
     }
     members = 1;
     parts = 0;
     if (a.n <= 32 && whole > 0) {
-      const int units = mine.blocks * a.nkv;
+      const int own = mine.blocks * a.nkv;
       const int least = max(a.least_tiles, (whole + there - 1) / there);
       for (int tiles = least; tiles <= least + SPARE_TILES; ++tiles) {
-        const int each_unit = (mine.tiles + tiles - 1) / tiles, blocks = units * each_unit;
+        const int each_unit = (mine.tiles + tiles - 1) / tiles, blocks = own * each_unit;
         if ((int)__reduce_add_sync(0xffffffffu, blocks) > there) continue;
         int upto = blocks;
 #pragma unroll
@@ -172,10 +181,15 @@ struct Walk {
       const int used = there / most * most;
       if ((float)whole * there >= 0.9f * (float)single * most * used && (float)whole >= 0.9f * (float)single * most) members = most;
     }
-    const int total = members > 1 ? single : whole;
+    if (members == 1) {
+      // whole units, where the longest share of them is no longer than tiles, beginnings and the merge of shares of tiles
+      const float rounds = (units + there - 1) / there;
+      if (rounds * (longest + BEGIN_TILES) < (float)whole / there + BEGIN_TILES * ((float)units / there + 2.f)) members = 0;
+    }
+    const int total = members > 1 ? single : members == 1 ? whole : units;
     const int share = members > 1 ? blockIdx.x / members : blockIdx.x;
-    member = blockIdx.x - share * members;
-    const int shares = min((total + a.least_tiles - 1) / a.least_tiles, there / members);
+    member = members > 1 ? blockIdx.x - share * members : 0;
+    const int shares = members > 0 ? min((total + a.least_tiles - 1) / a.least_tiles, there / members) : min(total, there);
     at = end = base = e = each = more = 0;
     if (share >= shares) return;
     each = total / shares;
@@ -226,8 +240,15 @@ struct Walk {
         base += weight(a, x);
         x = entry_of<ROWS, KEYS>(a, ++e);        // (at is below the total: such an entry is there)
       }
-      const int unit = (at - base) / x.tiles, t = at - base - unit * x.tiles, count = min(end - at, x.tiles - t);
-      at += count;
+      int unit, t = 0, count = x.tiles;
+      if (members > 0) {
+        unit = (at - base) / x.tiles;
+        t = at - base - unit * x.tiles;
+        count = min(end - at, x.tiles - t);
+        at += count;
+      } else {
+        unit = at++ - base;
+      }
       if (member >= x.blocks) continue;          // a block of rows that this entry does not have
       p.x = x;
       p.e = e;
@@ -432,8 +453,12 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) tree_merge_kernel(const __gr
   for (int i = 0; i < MERGE_DIMS; ++i)
     if (i < dims) dst[i] = from_float<T>(acc[i]);
 }
-template <typename T, int ROWS>
+// Not launched where no unit can have several slabs: every unit has at most least_tiles tiles by the block table's width, and there
+// are no more units than blocks (their parts are whole units then).
+template <typename T, int ROWS, int KEYS>
 inline void launch_merge(const Args& a, int blocks, cudaStream_t stream) {
+  const long long keys = (long long)a.table_stride * a.page_size, units = (long long)a.n * a.nkv * ((a.max_q_len * a.g + ROWS - 1) / ROWS);
+  if (a.n <= 32 && units <= blocks && (keys + KEYS - 1) / KEYS <= a.least_tiles) return;
   constexpr int RL = ROWS < 32 ? ROWS : 32, SPAN = 32 / RL * MERGE_DIMS;
   const int dim_warps = (a.hd + SPAN - 1) / SPAN, turns = std::min(MERGE_TURNS, MERGE_WARPS / dim_warps);
   const int max_rows = std::min(a.max_q_len * a.g, ROWS);

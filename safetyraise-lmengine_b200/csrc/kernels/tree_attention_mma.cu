@@ -321,7 +321,7 @@ static int run_form(const Args& a, int blocks, cudaStream_t stream) {
   const cudaError_t e = allow_smem((const void*)tree_mma_kernel<HD_MAX, KEY_WARPS, STAGES>, smem, have);
   if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", smem);
   launch_pdl(tree_mma_kernel<HD_MAX, KEY_WARPS, STAGES>, dim3(blocks), dim3(M_THREADS), smem, stream, a);
-  launch_merge<bf16, F::ROWS>(a, blocks, stream);
+  launch_merge<bf16, F::ROWS, M_KEYS>(a, blocks, stream);
   return launched();
 }
 // Stages: as many as leave room for another block on the SM.

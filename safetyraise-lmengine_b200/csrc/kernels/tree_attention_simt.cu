@@ -271,7 +271,7 @@ static int run_form(const Args& a, int blocks, cudaStream_t stream) {
   const cudaError_t e = allow_smem((const void*)tree_simt_kernel<T, DIMS, COPY, KEY_WARPS>, smem, have);
   if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", smem);
   launch_pdl(tree_simt_kernel<T, DIMS, COPY, KEY_WARPS>, dim3(blocks), dim3(S_THREADS), smem, stream, a);
-  launch_merge<T, SimtForm<KEY_WARPS>::ROWS>(a, blocks, stream);
+  launch_merge<T, SimtForm<KEY_WARPS>::ROWS, S_KEYS>(a, blocks, stream);
   return launched();
 }
 template <typename T, int DIMS, bool COPY>

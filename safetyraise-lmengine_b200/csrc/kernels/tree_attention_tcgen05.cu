@@ -508,7 +508,7 @@ static int run_form(const Args& a, int sms, cudaStream_t stream) {
   const cudaError_t e = allow_smem((const void*)tree_tcgen05_kernel<HD>, TmaForm<HD>::SMEM, have);
   if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", TmaForm<HD>::SMEM);
   launch_pdl(tree_tcgen05_kernel<HD>, dim3(sms), dim3(T_THREADS), TmaForm<HD>::SMEM, stream, mk, mv, a);
-  launch_merge<bf16, T_ROWS>(a, sms, stream);
+  launch_merge<bf16, T_ROWS, T_KEYS>(a, sms, stream);
   return launched();
 }
 int run_tcgen05(const Args& a, int sms, cudaStream_t stream) {

@@ -551,9 +551,9 @@ class Engine:
         with torch.cuda.device(self.mctx.device):
             from ..kernels import ops
             ctx = self._context(prep)
-            targets = self.workspace.get("drafts.targets", T, 1, torch.int32).view(T)
+            targets = torch.empty(T, dtype=torch.int32, device=self.mctx.device)
             ops.argmax(logits, targets, self.status[FAULT_LOGITS:FAULT_LOGITS + 1])
-            kept = self.workspace.get("drafts.kept", n, room + 2, torch.int32).view(-1)[:n * (room + 2)]
+            kept = torch.empty(n * (room + 2), dtype=torch.int32, device=self.mctx.device)
             path, count, following = kept[2 * n:].view(n, room), kept[:n], kept[n:2 * n]
             ops.accept_drafts(ctx.token_ids, ctx.parents, targets, ctx.cu_q, path, count, following)
             for g in self.cache.paged_groups:

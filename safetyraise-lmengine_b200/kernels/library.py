@@ -944,7 +944,6 @@ class KernelLibrary:
         self._check(self._entry("srlm_tree_attention")(
             *args, code, pages, *ints, n, T, nq, nkv, hd, page_size, scale, window, max_q_len, work.data_ptr(), sms,
             self._gemm_state(q.device)[1].data_ptr(), self._raw_stream(here)), what)
-        self.launches += 1               # the kernel that adds the shares
 
     def accept_drafts(self, tokens, parents, targets, cu_q, path, count, next_token):
         """Follows the model's own choice down each entry's tree of drafted tokens.

@@ -153,7 +153,7 @@ class StepContext:
         key = ("draft_mask", window)
         if key not in self.tables:
             from ..kernels import ops
-            mask = self.workspace.get(f"drafts.mask{window}", self.T, -(-self.max_q_len // 32), torch.int32)
+            mask = torch.empty((self.T, -(-self.max_q_len // 32)), dtype=torch.int32, device=self.positions.device)
             ops.draft_tree(self.parents, self.cu_q, self.kv_lens, self.positions, mask, window)
             self.tables[key] = mask
         return self.tables[key]
