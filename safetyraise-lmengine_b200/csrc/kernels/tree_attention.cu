@@ -54,14 +54,15 @@ extern "C" int srlm_tree_attention(const void* q, const void* k_cache, const voi
                nq, nkv, nq / nkv, hd, page_size, (int)num_pages, scale * 1.4426950408889634f,
                2.f * hd * (dtype == DT_F32 ? 4 : 2), window, 1, err_flag, work,
                ml, reinterpret_cast<int4*>(ml + 4ll * f.blocks * f.rows)};
-  if (kind != SIMT) {
-    if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) % 16)
-      return refuse(ST_BAD_ALIGN, "tree_attention: bfloat16 tensors start on 16-byte boundaries");
-    // (8 KV heads, 16 or 32 rows, us, tiles of 1 | 2 | 4 at least: tcgen05 behind 200 keys 12.3 | 10.6 | 10.5, behind 2,000 16.6 | 14.7 |
-    // 15.8; warp level 11.1 | 12.3 | 15.4 and 18.0 | 15.0 | 15.1; float32 13.3 | 15.0 | 18.7 and 22.5 | 20.4 | 22.0)
-    a.least_tiles = 2;
-    return kind == TCGEN05 ? tree::run_tcgen05(a, sms, stream) : tree::run_mma(a, max_rows, sms, stream);
-  }
-  a.least_tiles = 2;
-  return tree::run_simt(a, dtype, max_rows, sms, stream);
+  // A unit of few tiles by the block table's width is not divided: its last tiles take less than the merge and its launch (3.5 us of the
+  // host's time besides; us, divided | not: tcgen05 behind 300 keys 12.6 | 10.6, 500 12.0 | 11.0, 800 13.1 | 14.4; warp level behind 120
+  // 9.4 | 8.1, 200 9.8 | 10.0, 300 10.0 | 11.3; float32 behind 120 11.8 | 13.5).  Else parts and
+  // shares have two tiles at least (8 KV heads, 16 or 32 rows, us, 1 | 2 | 4: tcgen05 behind 200 keys 12.3 | 10.6 | 10.5, behind 2,000
+  // 16.6 | 14.7 | 15.8; warp level 11.1 | 12.3 | 15.4 and 18.0 | 15.0 | 15.1; float32 13.3 | 15.0 | 18.7 and 22.5 | 20.4 | 22.0).
+  const long long keys = (long long)table_stride * page_size, most = (keys + f.keys - 1) / f.keys;
+  a.least_tiles = most <= (kind == TCGEN05 ? 6 : kind == MMA ? 4 : 2) ? (int)most : 2;
+  if (kind == SIMT) return tree::run_simt(a, dtype, max_rows, sms, stream);
+  if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) % 16)
+    return refuse(ST_BAD_ALIGN, "tree_attention: bfloat16 tensors start on 16-byte boundaries");
+  return kind == TCGEN05 ? tree::run_tcgen05(a, sms, stream) : tree::run_mma(a, max_rows, sms, stream);
 }

@@ -312,8 +312,8 @@ __device__ __forceinline__ long long row_of_key(const Args& a, const int* table,
 }
 
 // Values that are no numbers, in tiles where rows see different keys.  A product multiplies a value that a row does not see by
-// zero, which leaves nothing of a finite one alone: such values are taken out of the tile (take_loose: eight bfloat16 numbers;
-// whether there was one) and the rows that see them get them back as they are written (loose_values).
+// zero, which leaves nothing of a finite one alone: such values are taken out of the tile (take_loose: eight bfloat16 numbers or four
+// float32 ones; whether there was one) and the rows that see them get them back as they are written (loose_values).
 __device__ __forceinline__ bool take_loose(uint4& v) {
   uint32_t* w = reinterpret_cast<uint32_t*>(&v);
   bool here = false;
@@ -327,14 +327,26 @@ __device__ __forceinline__ bool take_loose(uint4& v) {
   return here;
 }
 
+__device__ __forceinline__ bool take_loose(float4& v) {
+  bool here = false;
+  float* f = reinterpret_cast<float*>(&v);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (!isfinite(f[k])) {
+      f[k] = 0.f;
+      here = true;
+    }
+  return here;
+}
+
 // The sum of the non-finite values of dimension d that a row sees in the piece's masked tiles (all tiles are looked through: this is
 // for rows whose cache holds such values).
-template <int KEYS>
+template <typename T, int KEYS>
 __device__ __noinline__ float loose_values(const Args& a, int start, int kv_len, const int* table, int kvh, int token, int d, int tile_lo,
                                            int tile_hi) {
   float sum = 0.f;
   const int lo = first_key_of(a, token, start);
-  const bf16* v = (const bf16*)a.v_cache;
+  const T* v = (const T*)a.v_cache;
   for (int j0 = tile_lo * KEYS; j0 < tile_hi * KEYS && j0 < kv_len; j0 += 32) {
     if (j0 / KEYS * KEYS + KEYS <= start && (a.window <= 0 || j0 / KEYS * KEYS >= kv_len - a.window)) continue;
     Sight<1> sight;

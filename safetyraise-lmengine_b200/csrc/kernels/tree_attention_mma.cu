@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
     if (loose) {                                                 // (what a row sees of them outweighs all the rest)
       for (int i = tid; i < rows * hd; i += M_THREADS) {
         const int row = i / hd, d = i - row * hd;
-        const float v = loose_values<M_KEYS>(a, x.start, x.kv_len, table, w.kvh, x.q0 + (r0 + row) / g, d, w.tile_lo, w.tile_hi);
+        const float v = loose_values<bf16, M_KEYS>(a, x.start, x.kv_len, table, w.kvh, x.q0 + (r0 + row) / g, d, w.tile_lo, w.tile_hi);
         if (isfinite(v)) continue;
         if (whole) out_of(row)[d] = from_float<bf16>(v);
         else a.part_o[(slab * hd + d) * ROWS + row] = v;

@@ -8,10 +8,7 @@
 // keys times groups of its rows, so that a row's maximum and sum are reductions over lanes; for the outputs a lane holds the
 // dimensions lane + 32 i, so that nothing but the weights passes through shared memory.  Bound by the latency of the FMAs' operands
 // from shared memory (a 16-byte read feeds 32 of them at best), which more warps on the SM hide.
-// A masked key's weight is an exact zero and its value is not multiplied: what stands in a place that a row does not see
-// never reaches it.
-#include <type_traits>
-
+// A masked key's weight is an exact zero; values that are no numbers are taken out of tiles in which rows see different keys.
 #include "tree_attention.cuh"
 
 namespace srlm {
@@ -40,6 +37,7 @@ __global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const __grid_const
   float* p_sh = q_sh + ROWS * ld;                          // [warps][8][WK] weights
   float* f_sh = p_sh + S_WARPS * S_OWN * WK;               // [warps][8] what the rows' sums so far are multiplied by
   long long* at_sh = reinterpret_cast<long long*>(f_sh + S_WARPS * S_OWN);      // [3][keys]: first element of a key's row; -1: none
+  __shared__ int loose_sh;
   const T* q = (const T*)a.q;
   const T* kc = (const T*)a.k_cache;
   const T* vc = (const T*)a.v_cache;
@@ -92,9 +90,21 @@ __global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const __grid_const
     };
     locate(0);
     locate(1);
-    for (int i = tid; i < ROWS * ld; i += S_THREADS) {
-      const int row = i / ld, d = i - row * ld, r = r0 + row;
-      q_sh[i] = row < rows && d < a.hd ? to_float(q[((size_t)(x.q0 + r / g) * a.nq + w.kvh * g + r % g) * a.hd + d]) : 0.f;
+    if (tid == 0) loose_sh = 0;
+    if (COPY && ((uintptr_t)a.q & 15) == 0) {              // (in the first tile's group: there before it is read)
+      for (int i = tid; i < ROWS * pieces; i += S_THREADS) {
+        const int row = i / pieces, c = (i - row * pieces) * 4, r = r0 + row;
+        const bool there = row < rows;
+        const unsigned at = (unsigned)__cvta_generic_to_shared(q_sh + row * ld + c);
+        const T* src = there ? q + ((size_t)(x.q0 + r / g) * a.nq + w.kvh * g + r % g) * a.hd + c : q;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(src), "r"(there ? 16 : 0) : "memory");
+      }
+    } else {
+#pragma unroll 8
+      for (int i = tid; i < ROWS * ld; i += S_THREADS) {
+        const int row = i / ld, d = i - row * ld, r = r0 + row;
+        q_sh[i] = row < rows && d < a.hd ? to_float(q[((size_t)(x.q0 + r / g) * a.nq + w.kvh * g + r % g) * a.hd + d]) : 0.f;
+      }
     }
     __syncthreads();
     fetch(0);
@@ -117,6 +127,19 @@ __global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const __grid_const
       __syncthreads();
       // every row sees every key of a tile between the window's last edge and the drafted tokens
       const bool plain = j0 + S_KEYS <= x.start && (a.window <= 0 || j0 >= x.kv_len - a.window);
+      if (!plain) {
+        bool loose = false;
+        for (int i = tid; i < S_KEYS * pieces; i += S_THREADS) {
+          float4* p = reinterpret_cast<float4*>(v_sh + ((t & 1) * S_KEYS + i / pieces) * ld + i % pieces * 4);
+          float4 v = *p;
+          if (take_loose(v)) {
+            *p = v;
+            loose = true;
+          }
+        }
+        if (loose) loose_sh = 1;
+        __syncthreads();
+      }
       if (live) {
         const float4* kp = reinterpret_cast<const float4*>(k_sh + ((t & 1) * S_KEYS + key) * ld);
         const float4* qp = reinterpret_cast<const float4*>(q_sh + rows0 * ld);
@@ -173,27 +196,23 @@ __global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const __grid_const
           for (int i = 0; i < DIMS; ++i) acc[o][i] *= f;
         }
         const float* vp = v_sh + ((t & 1) * S_KEYS + key0) * ld + lane;
-        auto add = [&](auto tested) {
 #pragma unroll 1
-          for (int jj = 0; jj < WK; jj += 4) {
-            float v[4][DIMS];
+        for (int jj = 0; jj < WK; jj += 4) {
+          float v[4][DIMS];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int i = 0; i < DIMS; ++i) v[e][i] = lane + 32 * i < ld ? vp[(jj + e) * ld + 32 * i] : 0.f;
+#pragma unroll
+          for (int o = 0; o < S_OWN; ++o) {
+            const float4 p4 = *reinterpret_cast<const float4*>(p_own + o * WK + jj);
+            const float p[4] = {p4.x, p4.y, p4.z, p4.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-              for (int i = 0; i < DIMS; ++i) v[e][i] = lane + 32 * i < ld ? vp[(jj + e) * ld + 32 * i] : 0.f;
-#pragma unroll
-            for (int o = 0; o < S_OWN; ++o) {
-              const float4 p4 = *reinterpret_cast<const float4*>(p_own + o * WK + jj);
-              const float p[4] = {p4.x, p4.y, p4.z, p4.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (!decltype(tested)::value || p[e] != 0.f)
-#pragma unroll
-                  for (int i = 0; i < DIMS; ++i) acc[o][i] = fmaf(p[e], v[e][i], acc[o][i]);
-            }
+              for (int i = 0; i < DIMS; ++i) acc[o][i] = fmaf(p[e], v[e][i], acc[o][i]);
           }
-        };
-        if (plain) add(std::false_type{}); else add(std::true_type{});
+        }
       }
       __syncthreads();
     }
@@ -253,6 +272,18 @@ __global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const __grid_const
       }
     }
     __syncthreads();                                       // before the next piece's places and rows
+    if (loose_sh) {                                        // (what a row sees of them outweighs all the rest)
+      const bool whole = w.begins && w.ends;
+      const size_t slab = slab_of(blockIdx.x, w.begins);
+      for (int i = tid; i < rows * a.hd; i += S_THREADS) {
+        const int row = i / a.hd, d = i - row * a.hd, r = r0 + row;
+        const float v = loose_values<T, S_KEYS>(a, x.start, x.kv_len, table, w.kvh, x.q0 + r / g, d, w.tile_lo, w.tile_hi);
+        if (isfinite(v)) continue;
+        if (whole) ((T*)a.out)[((size_t)(x.q0 + r / g) * a.nq + w.kvh * g + r % g) * a.hd + d] = from_float<T>(v);
+        else a.part_o[(slab * a.hd + d) * ROWS + row] = v;
+      }
+      __syncthreads();
+    }
   }
 }
 
