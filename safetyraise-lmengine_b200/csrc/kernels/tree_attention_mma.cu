@@ -36,8 +36,11 @@ struct MmaForm {
   }
 };
 
+// Blocks on an SM, by registers and shared memory: the grid is what runs at once.
+__host__ __device__ constexpr int mma_blocks(int hd) { return hd <= 64 ? 3 : hd <= 128 ? 2 : 1; }
+
 template <int HD_MAX, int KEY_WARPS, int STAGES>
-__global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(M_THREADS, mma_blocks(HD_MAX)) tree_mma_kernel(const __grid_constant__ Args a) {
   using Form = MmaForm<HD_MAX, KEY_WARPS, STAGES>;
   constexpr int ROWS = Form::ROWS, WK = M_KEYS / KEY_WARPS;      // keys of a warp in a tile
   constexpr int KS = HD_MAX / 16, NO = HD_MAX / 8, NS = WK / 8;
@@ -308,10 +311,9 @@ __global__ void __launch_bounds__(M_THREADS) tree_mma_kernel(const __grid_consta
 // Warps along the keys: by the rows that an entry has at most (8 KV heads of 128, pages of 20, 8 entries behind 8,000 keys, us, four |
 // two | one: 16 rows 60.7 | 63.0 | 68.9, 32 rows 104 | 65.5 | 77.6, 64 rows 183 | 114 | 83.2).
 static int key_warps(int max_rows) { return max_rows <= 16 ? 4 : max_rows <= 32 ? 2 : 1; }
-static int blocks_per_sm(int hd) { return hd <= 64 ? 3 : hd <= 128 ? 2 : 1; }
 
 bool mma_takes(int hd) { return hd % 16 == 0 && hd <= 256; }
-Form mma_form(int hd, int max_rows, int sms) { return Form{blocks_per_sm(hd) * sms, 64 / key_warps(max_rows), M_KEYS}; }
+Form mma_form(int hd, int max_rows, int sms) { return Form{mma_blocks(hd) * sms, 64 / key_warps(max_rows), M_KEYS}; }
 
 template <int HD_MAX, int KEY_WARPS, int STAGES>
 static int run_form(const Args& a, int blocks, cudaStream_t stream) {

@@ -25,8 +25,12 @@ struct SimtForm {
   }
 };
 
+// Blocks on an SM: the grid is what runs at once (heads of up to 64, all rows: three, of 168 registers; a fourth wave of blocks that do
+// not fit took a quarter longer: 64 rows behind 4,000 keys, 16 entries, 389 | 306 us).
+__host__ __device__ constexpr int simt_blocks(int dims, int key_warps) { return dims == 2 ? (key_warps == 1 ? 3 : 4) : dims == 4 ? 2 : 1; }
+
 template <typename T, int DIMS, bool COPY, int KEY_WARPS>
-__global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(S_THREADS, simt_blocks(DIMS, KEY_WARPS)) tree_simt_kernel(const __grid_constant__ Args a) {
   using Form = SimtForm<KEY_WARPS>;
   constexpr int ROWS = Form::ROWS, WK = Form::WK, PER = Form::PER;
   extern __shared__ __align__(16) float tree_sh[];
@@ -292,7 +296,7 @@ __global__ void __launch_bounds__(S_THREADS) tree_simt_kernel(const __grid_const
 static int key_warps(int max_rows) { return max_rows <= 8 ? 4 : max_rows <= 16 ? 2 : 1; }
 
 Form simt_form(int hd, int max_rows, int sms) {
-  return Form{(hd <= 64 ? 4 : hd <= 128 ? 2 : 1) * sms, S_OWN * S_WARPS / key_warps(max_rows), S_KEYS};
+  return Form{simt_blocks(hd <= 64 ? 2 : hd <= 128 ? 4 : 8, key_warps(max_rows)) * sms, S_OWN * S_WARPS / key_warps(max_rows), S_KEYS};
 }
 
 template <typename T, int DIMS, bool COPY, int KEY_WARPS>
