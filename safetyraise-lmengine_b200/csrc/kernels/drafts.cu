@@ -10,6 +10,10 @@ namespace drafts {
 
 enum ErrorCode : int { ERR_PARENT = 73, ERR_PATH = 74 };
 
+// An entry's tokens, or -1 where its bounds are none of T rows: compared before they are subtracted, for a difference of wild
+// numbers may pass 32 bits and look right again.
+__device__ __forceinline__ int tokens_of(int q0, int q1, int T) { return q0 >= 0 && q1 >= q0 && q1 <= T ? q1 - q0 : -1; }
+
 // ---------------------------------------------------------------------------
 // positions[t] = committed tokens + depth of t, and bit k of mask[t]: k is t or one of its ancestors (at most window - 1 above
 // it, where there is a window).  A thread a token: it goes up its line, whose numbers fall, and writes its words from the last
@@ -24,11 +28,12 @@ __global__ void __launch_bounds__(TREE_THREADS) draft_tree_kernel(const int* __r
   pdl_wait();
   pdl_trigger();
   const int e = blockIdx.x;
-  const int q0 = cu_q[e], q_len = cu_q[e + 1] - q0, start = kv_lens[e] - q_len;
-  if (q0 < 0 || q_len <= 0 || q0 + q_len > T || q_len > 32 * words || start < 0) {
+  const int q0 = cu_q[e], q_len = tokens_of(q0, cu_q[e + 1], T), kv_len = kv_lens[e];
+  if (q_len <= 0 || q_len > 32ll * words || kv_len < q_len) {
     if (q_len != 0 && threadIdx.x == 0) atomicExch(err, ERR_PARENT);
     return;
   }
+  const int start = kv_len - q_len;
   const int* up = parents + q0;
   for (int i = blockIdx.y * TREE_THREADS + threadIdx.x; i < q_len; i += gridDim.y * TREE_THREADS) {
     int* row = mask + (size_t)(q0 + i) * words;
@@ -68,9 +73,9 @@ __global__ void __launch_bounds__(32) accept_drafts_kernel(const int* __restrict
   pdl_wait();
   pdl_trigger();
   const int e = blockIdx.x, lane = threadIdx.x;
-  const int q0 = cu_q[e], q_len = cu_q[e + 1] - q0;
+  const int q0 = cu_q[e], q_len = tokens_of(q0, cu_q[e + 1], T);
   int* line = path + (size_t)e * cap;
-  if (q0 < 0 || q_len <= 0 || q0 + q_len > T) {
+  if (q_len <= 0) {
     if (lane == 0) {
       if (q_len != 0) atomicExch(err, ERR_PARENT);
       count[e] = 0;
@@ -124,7 +129,7 @@ __global__ void __launch_bounds__(KEEP_THREADS) keep_drafts_kernel(V* __restrict
   pdl_wait();
   pdl_trigger();
   const int e = blockIdx.y;
-  const int q_len = cu_q[e + 1] - cu_q[e], start = kv_lens[e] - q_len, kept = min(count[e], cap);
+  const int q_len = tokens_of(cu_q[e], cu_q[e + 1], 0x7fffffff), kv_len = kv_lens[e], kept = min(count[e], cap);
   const int* line = path + (size_t)e * cap;
   const int* table = block_table + (size_t)e * table_stride;
   const long long per_slab = (long long)nkv * row_pieces, columns = slabs * per_slab;
@@ -137,9 +142,9 @@ __global__ void __launch_bounds__(KEEP_THREADS) keep_drafts_kernel(V* __restrict
     for (int i = threadIdx.x; i < rows; i += KEEP_THREADS) {
       const int k = line[i0 + i], before = i0 + i > 0 ? line[i0 + i - 1] : -1;
       long long at[2] = {-1, -1};
-      bool good = start >= 0 && k >= i0 + i && k > before && k < q_len;
+      bool good = q_len >= 0 && kv_len >= q_len && k >= i0 + i && k > before && k < q_len;
       for (int s = 0; s < 2 && good; ++s) {
-        const int place = start + (s ? i0 + i : k), pg = place / page_size;
+        const int place = kv_len - q_len + (s ? i0 + i : k), pg = place / page_size;
         const int page = pg < table_stride ? table[pg] : -1;
         good = page >= 0 && page < num_pages;
         at[s] = ((long long)page * nkv * page_size + (place - pg * page_size)) * row_pieces;

@@ -16,9 +16,6 @@
 // weights (a slab per block: it has at most one unit that began before it and one that goes on behind it), which
 // tree_merge_kernel adds in the order of the keys.  The sums depend on the lengths and C alone.
 // Small work is divided along the units instead: each into as many equal parts as keep every block at one part.  A block whose
-// share reaches into a second unit begins anew with its rows and its first keys, which costs it SPARE_TILES tiles' time (8 entries of
-// 128 rows behind 2,000 keys, 8 KV heads: 33.8 us by shares of all tiles, 29.5 by parts of units).
-// Small work is divided along the units instead: each into as many equal parts as keep every block at one part.  A block whose
 // share reaches into a second unit begins anew with its rows and its first keys and leaves two slabs, which costs it more than
 // SPARE_TILES tiles (entries of 128 rows, 8 KV heads of 128, us, shares of all tiles | parts: 1 behind 600 keys 22.1 | 15.8, 8
 // behind 2,000 29.9 | 25.8, 16 behind 2,000 51.5 | 34.7, 16 behind 4,000 68.1 | 56.0, 12 behind 8,000 77.0 | 82.5, which is beyond
@@ -82,16 +79,19 @@ template <int ROWS, int KEYS>
 __device__ __forceinline__ Entry entry_of(const Args& a, int e, bool flag = false) {
   Entry x;
   x.q0 = a.cu_q[e];
-  x.q_len = a.cu_q[e + 1] - x.q0;
+  const int q1 = a.cu_q[e + 1];
   x.kv_len = a.kv_lens[e];
-  x.start = x.kv_len - x.q_len;
-  const bool good = x.q_len >= 0 && x.q0 >= 0 && x.q0 + x.q_len <= a.T && x.start >= 0 && x.q_len <= a.max_q_len &&
+  // compared before they are subtracted: a difference of wild numbers may pass 32 bits and look right again
+  const bool rows = x.q0 >= 0 && q1 >= x.q0 && q1 <= a.T;
+  x.q_len = rows ? q1 - x.q0 : 0;
+  const bool good = rows && x.q_len <= a.max_q_len && x.kv_len >= x.q_len &&
                     x.kv_len <= (long long)a.table_stride * a.page_size;
   if (!good || x.q_len == 0) {
     if (!good && flag) atomicExch(a.err_flag, ERR_ENTRY);
-    x.q_len = x.tiles = x.blocks = x.first_tile = 0;
+    x.q_len = x.start = x.tiles = x.blocks = x.first_tile = 0;
     return x;
   }
+  x.start = x.kv_len - x.q_len;
   // no row's position is below start
   const int first = a.window > 0 ? max(0, x.start - a.window + 1) : 0;
   x.first_tile = first / KEYS;

@@ -358,6 +358,41 @@ def test_bad_pages_and_lengths_raise_the_error_word():
         assert torch.equal(c.out[:9], good[:9]) and (c.out[9:] == 7.0).all()
 
 
+def test_lengths_whose_sums_pass_32_bits_raise_the_error_word():
+    """Differences and sums of such lengths come out as numbers that would do."""
+    low, high = -2 ** 31, 2 ** 31 - 1
+    ops.gemm_error_flag(torch.device(DEV))
+    for dt, hd in ((torch.float32, 64), (torch.bfloat16, 128), (torch.bfloat16, 32)):
+        c = Case([9, 20], [100, 30], 8, 2, hd, 16, dt, seed=1)
+        good = c.run().clone()
+        for kv in (low, low + 3, low + 8):                         # less 9 tokens: 2^31 - 9 and so on
+            c.kv_lens[0] = kv
+            c.out.fill_(7.0)
+            c.run()
+            assert ops.gemm_error_flag(torch.device(DEV)) != 0
+            assert (c.out[:9] == 7.0).all() and torch.equal(c.out[9:], good[9:])
+        c.kv_lens[0] = c.kv[0]
+        c.cu_q.copy_(ints([high - 3, low + 5, low + 14]))          # entry 0: 9 tokens from 2^31 - 4 on; entry 1: below none
+        c.out.fill_(7.0)
+        c.run()
+        assert ops.gemm_error_flag(torch.device(DEV)) != 0 and (c.out == 7.0).all()
+    parents, cu = ints([-1, 0, 1, 2, 3]), ints([0, 5])
+    for lens, kv in (([0, 5], low), ([0, 5], low + 4), ([high - 1, low + 3], 100)):
+        positions, mask = ints([7] * 5), ints([[7]] * 5)
+        ops.draft_tree(parents, ints(lens), ints([kv]), positions, mask)
+        assert ops.gemm_error_flag(torch.device(DEV)) != 0
+        assert (positions == 7).all() and (mask == 7).all()
+    path, count, following = ints([[7] * 5]), ints([7]), ints([7])
+    ops.accept_drafts(parents, parents, parents, ints([high - 1, low + 3]), path, count, following)
+    assert ops.gemm_error_flag(torch.device(DEV)) != 0
+    assert (path == -1).all() and int(count) == 0 and int(following) == -1
+    for lens, kv in (([0, 5], low), ([0, 5], low + 4), ([0, -5], 100), ([0, 5], 4)):
+        pool = torch.randn(2, 4, 1, 4, 8, device=DEV)
+        was = pool.clone()
+        ops.keep_drafts(pool, ints([[1, 2]]), ints(lens), ints([kv]), ints([[0, 2, 4]]), ints([3]))
+        assert ops.gemm_error_flag(torch.device(DEV)) != 0 and torch.equal(pool, was)
+
+
 @pytest.mark.parametrize("lens, chain, window", [([1], False, 0), ([7, 1, 32, 33], False, 0), ([200, 64, 90], False, 5), ([130, 31], True, 0),
                                                  ([130], True, 1), ([40, 256], True, 33)])
 def test_draft_tree(lens, chain, window):
