@@ -44,9 +44,9 @@ extern "C" int srlm_tree_attention(const void* q, const void* k_cache, const voi
   const int max_rows = max_q_len * (nq / nkv);
   const Kind kind = kind_of(dtype, hd, page_size);
   const tree::Form f = form_of(kind, hd, max_rows, sms);
-  // the list of all units' tiles is counted in 31 bits
+  // the list of all units' tiles is counted in 31 bits, and so are an entry's keys with a tile to spare
   const double units = (double)n * nkv * ((double)max_q_len * (nq / nkv) / f.rows + 1), tiles = (double)table_stride * page_size / f.keys + 1;
-  if (units * tiles > 2147483647.0)
+  if (units * tiles > 2147483647.0 || (long long)table_stride * page_size > (1 << 30))
     return refuse(ST_BAD_SIZE, "tree_attention: %d entries of up to %d tokens and %d pages are more work than a call takes", n, max_q_len,
                   table_stride);
   float* ml = work + 2ll * f.blocks * f.rows * hd;      // (sizes are multiples of 16 bytes)

@@ -228,8 +228,10 @@ struct Walk {
       p.e = e;
       p.kvh = at / x.blocks;
       p.block = at - p.kvh * x.blocks;
-      p.tile_lo = x.first_tile + base * x.tiles / parts;
-      p.tile_hi = x.first_tile + (base + 1) * x.tiles / parts;
+      // the first `longer` parts have a tile more (no product of parts and tiles: it would pass 32 bits)
+      const int part = x.tiles / parts, longer = x.tiles - part * parts;
+      p.tile_lo = x.first_tile + base * part + min(base, longer);
+      p.tile_hi = p.tile_lo + part + (base < longer ? 1 : 0);
       p.begins = base == 0;
       p.ends = base + 1 == parts;
       at = end;

@@ -547,6 +547,28 @@ def test_pages_far_into_a_pool():
     assert torch.equal(pool[far + 1, 0, 15], pool[2, 0, 2]) and torch.equal(pool[far + 2, 0, 0], pool[2, 0, 3])
 
 
+@pytest.mark.parametrize("dt, hd, keys", [(torch.float32, 16, 200_000_001), (torch.bfloat16, 16, 330_000_001), (torch.bfloat16, 64, 1 << 30)])
+def test_as_many_keys_as_an_entry_may_have(dt, hd, keys):
+    """One page over and over: parts times tiles pass 32 bits.  Scores are zero, so a weight is 1, sums of up to 2^24 of them
+    are exact in float32, and what comes out is the page's value."""
+    page = 512
+    k, v = torch.randn(1, 1, page, hd, device=DEV).to(dt), torch.full((1, 1, page, hd), 0.75, device=DEV, dtype=dt)
+    q, out = torch.zeros(1, hd, device=DEV, dtype=dt), torch.full((1, hd), 7.0, device=DEV, dtype=dt)
+    table = torch.zeros(1, -(-keys // page), dtype=torch.int32, device=DEV)
+    ops.gemm_error_flag(torch.device(DEV))
+    ops.tree_attention(q, k, v, out, table, ints([0, 1]), ints([keys]), ints([[1]]), 1, 1, hd, page, 1.0, 1)
+    assert ops.gemm_error_flag(torch.device(DEV)) == 0
+    # what is added of the parts, at most 1,200 of them, is off by 2^-24 each
+    assert (out.double() - 0.75).abs().max() <= 0.75 * (1200 * 2 * U + HALF[dt])
+
+
+def test_a_table_of_more_keys_than_an_entry_may_have_is_refused():
+    k = torch.zeros(1, 1, 1024, 16, device=DEV)
+    q = torch.zeros(1, 16, device=DEV)
+    with pytest.raises(Exception, match="more work than a call takes"):
+        ops.tree_attention(q, k, k, q.clone(), ints(np.zeros((1, (1 << 20) + 1))), ints([0, 1]), ints([5]), ints([[1]]), 1, 1, 16, 1024, 1.0, 1)
+
+
 def test_a_verification_as_it_is_used():
     """Mask, attention, the walk and the move, in a row and in a graph: the kept rows are the accepted tokens', and attention
     over them is that of the same tokens decoded one behind another."""
