@@ -548,19 +548,23 @@ class Engine:
         prep = self.prepare([StepEntry(e.slot, e.tokens, range(len(e.tokens)), e.generation, e.parents) for e in entries], drafts=True)
         logits = self.launch(prep)
         n, room, T = len(entries), max(prep.q_lens), sum(prep.q_lens)
-        with torch.cuda.device(self.mctx.device):
-            from ..kernels import ops
-            ctx = self._context(prep)
-            targets = torch.empty(T, dtype=torch.int32, device=self.mctx.device)
-            ops.argmax(logits, targets, self.status[FAULT_LOGITS:FAULT_LOGITS + 1])
-            kept = torch.empty(n * (room + 2), dtype=torch.int32, device=self.mctx.device)
-            path, count, following = kept[2 * n:].view(n, room), kept[:n], kept[n:2 * n]
-            ops.accept_drafts(ctx.token_ids, ctx.parents, targets, ctx.cu_q, path, count, following)
-            for g in self.cache.paged_groups:
-                for pools in (self.cache.kv_pools, self.cache.k_pools, self.cache.v_pools):
-                    if g.name in pools:
-                        ops.keep_drafts(pools[g.name], ctx.block_tables[g.name], ctx.cu_q, ctx.kv_lens, path, count)
-            found = kept.tolist()
+        try:
+            with torch.cuda.device(self.mctx.device):
+                from ..kernels import ops
+                ctx = self._context(prep)
+                targets = torch.empty(T, dtype=torch.int32, device=self.mctx.device)
+                ops.argmax(logits, targets, self.status[FAULT_LOGITS:FAULT_LOGITS + 1])
+                kept = torch.empty(n * (room + 2), dtype=torch.int32, device=self.mctx.device)
+                path, count, following = kept[2 * n:].view(n, room), kept[:n], kept[n:2 * n]
+                ops.accept_drafts(ctx.token_ids, ctx.parents, targets, ctx.cu_q, path, count, following)
+                for g in self.cache.paged_groups:
+                    for pools in (self.cache.kv_pools, self.cache.k_pools, self.cache.v_pools):
+                        if g.name in pools:
+                            ops.keep_drafts(pools[g.name], ctx.block_tables[g.name], ctx.cu_q, ctx.kv_lens, path, count)
+                found = kept.tolist()
+        except Exception:
+            self.revoke(prep)                             # nothing was committed: the reserved pages go back
+            raise
         fault = self.fault_of(self.read_faults())
         if fault is not None:
             self.revoke(prep)

@@ -180,6 +180,27 @@ def test_verify_refuses_and_fails_like_a_step(folder_a):
     assert np.abs(got - ref).max() <= TOL["float32"] * np.abs(ref).max()
 
 
+@pytest.mark.parametrize("name", ["argmax", "accept_drafts", "keep_drafts"])
+def test_an_error_on_the_host_behind_the_forward_keeps_nothing(folder_a, monkeypatch, name):
+    from safetyraise_lmengine_b200 import StepEntry
+    from safetyraise_lmengine_b200.kernels import ops
+    eng = build(folder_a, num_pages=6)
+    s = eng.open_request()
+    eng.step([StepEntry(s, [1, 2, 3, 4, 5])])
+    before = (eng.cache.length(s), eng.cache.free_pages())
+
+    def fails(*_, **__):
+        raise MemoryError("no memory")
+    with monkeypatch.context() as m:
+        m.setattr(ops, name, fails, raising=False)
+        with pytest.raises(MemoryError):
+            eng.verify([StepEntry(s, [6, 7, 8, 9, 10, 11, 12, 13], parents=[-1, 0, 0, 1, 1, 2, 2, 3])])
+    assert (eng.cache.length(s), eng.cache.free_pages()) == before and eng.cache.audit() == 0
+    got = eng.step([StepEntry(s, [6], [0])]).cpu().numpy()
+    ref = plain_logits(folder_a, [1, 2, 3, 4, 5, 6])[-1:]
+    assert np.abs(got - ref).max() <= TOL["float32"] * np.abs(ref).max()
+
+
 def test_other_mixers_refuse_drafts(tmp_path_factory):
     from safetyraise_lmengine_b200 import StepEntry
     from safetyraise_lmengine_b200.errors import Unsupported
