@@ -460,7 +460,8 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (loose_sh && mine)                      // (what a row sees of them outweighs all the rest)
 #pragma unroll 1
           for (int c = i * (HD / 2); c < (i + 1) * (HD / 2); ++c) {
-            const float v = loose_values<bf16, T_KEYS>(a, x.start, x.kv_len, a.block_table + (size_t)w.e * a.table_stride, w.kvh, token, c, w.tile_lo, w.tile_hi);
+            const float v = loose_values<bf16, T_KEYS>(a, x.start, x.kv_len, a.block_table + (size_t)w.e * a.table_stride, w.kvh, token,
+                                                       c, w.tile_lo, w.tile_hi);
             if (!isfinite(v)) {
               if (whole) dst[c] = from_float<bf16>(v);
               else a.part_o[(slab * HD + c) * T_ROWS + row] = v;
