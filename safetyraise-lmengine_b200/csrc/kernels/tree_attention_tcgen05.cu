@@ -363,6 +363,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           }
           if (loose) loose_sh = 1;
           fence_async_smem();
+          __syncwarp();                            // a warp of no rows arrives for all its lanes at once: each has written and fenced by then
         }
         if (live) {
           Row srow;
