@@ -210,11 +210,11 @@ __global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(V* __restrict_
   }
 }
 
-// bytes of the widest access that every row starts and ends on
+// bytes of the widest access that every row starts and ends on: two at least, for the entries refuse odd addresses and odd sizes
 static int piece_bytes(const void* p, long long row_bytes) {
-  for (int b = 16; b > 1; b >>= 1)
-    if ((uintptr_t)p % b == 0 && row_bytes % b == 0) return b;
-  return 1;
+  int b = 16;
+  while (b > 2 && ((uintptr_t)p % b || row_bytes % b)) b >>= 1;
+  return b;
 }
 template <typename F>
 static int with_pieces(int bytes, F f) {
@@ -287,6 +287,7 @@ extern "C" int srlm_keep_drafts(void* pool, long long slabs, long long num_pages
       n > 65535 || slabs > (1 << 20) || num_pages > 0x7fffffff || row_bytes > (1 << 20) || nkv > (1 << 20) || !err)
     return refuse(ST_BAD_SIZE, "keep_drafts: slabs=%lld pages=%lld nkv=%d page_size=%d row=%lld bytes entries=%d", slabs, num_pages, nkv,
                   page_size, row_bytes, n);
+  if ((uintptr_t)pool % 2) return refuse(ST_BAD_ALIGN, "keep_drafts: the pool starts on an odd address");
   const int bytes = piece_bytes(pool, row_bytes);
   const long long pieces = row_bytes / bytes, columns = slabs * nkv * pieces, blocks = (columns + KEEP_THREADS - 1) / KEEP_THREADS;
   if (blocks > 0x7fffffff) return refuse(ST_BAD_SIZE, "keep_drafts: %lld columns", columns);
@@ -305,6 +306,7 @@ extern "C" int srlm_copy_pages(void* pool, long long slabs, long long num_pages,
   if (n <= 0) return ST_OK;
   if (slabs <= 0 || num_pages <= 0 || num_pages > 0x7fffffff || page_bytes <= 0 || page_bytes % 2 || slabs > (1 << 20) || sms <= 0)
     return refuse(ST_BAD_SIZE, "copy_pages: slabs=%lld pages=%lld of %lld bytes", slabs, num_pages, page_bytes);
+  if ((uintptr_t)pool % 2) return refuse(ST_BAD_ALIGN, "copy_pages: the pool starts on an odd address");
   for (int i = 0; i < n; ++i)
     if (src[i] < 0 || src[i] >= num_pages || dst[i] < 0 || dst[i] >= num_pages)
       return refuse(ST_BAD_SIZE, "copy_pages: page %lld or %lld is outside the pool of %lld", src[i], dst[i], num_pages);

@@ -5,7 +5,9 @@ import math
 import pytest
 import torch
 
-from test_drafts_gpu import Case
+from safetyraise_lmengine_b200.errors import ShapeError
+from safetyraise_lmengine_b200.kernels import ops
+from test_drafts_gpu import DEV, Case, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +33,23 @@ def test_blocks_of_few_rows_beside_numbers_that_are_none(hd, ps, tokens, window)
             c.out.fill_(7.0)
             c.run()
             assert torch.equal(c.out, first)
+
+
+def test_pools_of_one_byte_numbers():
+    """Copied and moved at even addresses, refused at odd ones."""
+    flat = torch.randint(0, 256, (2 * 4 * 3 * 4 * 6 + 2,), dtype=torch.uint8, device=DEV)
+    for at in (0, 2):
+        pool = flat[at:at + 576].view(2, 4, 3, 4, 6)
+        want = pool.clone()
+        want[:, 3] = want[:, 1]
+        ops.copy_pages(pool, [1], [3])
+        assert torch.equal(pool, want)
+        want[:, 2, :, 1] = want[:, 2, :, 3]
+        ops.keep_drafts(pool, ints([[2]]), ints([0, 4]), ints([4]), ints([[0, 3]]), ints([2]))
+        assert torch.equal(pool, want)
+    was, pool = flat.clone(), flat[1:577].view(2, 4, 3, 4, 6)
+    with pytest.raises(ShapeError, match="odd address"):
+        ops.copy_pages(pool, [1], [3])
+    with pytest.raises(ShapeError, match="odd address"):
+        ops.keep_drafts(pool, ints([[2]]), ints([0, 4]), ints([4]), ints([[0, 3]]), ints([2]))
+    assert torch.equal(flat, was)
