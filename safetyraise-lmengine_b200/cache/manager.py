@@ -168,6 +168,7 @@ class CacheManager:
                     self.v_pools[g.name] = torch.zeros((len(g.entries), num_pages, g.kv_heads, page_size,
                                                         g.value_dim), dtype=dtype, device=device)
         self._table_buf = (C.c_int32 * (num_pages + 1))()
+        self._state_came: Dict[int, int] = {}     # slot -> the generation whose fixed-size state a fork brought
 
     def __del__(self):
         h, self._h = getattr(self, "_h", None), None
@@ -245,9 +246,15 @@ class CacheManager:
             raise ResourceExhausted(f"no free page for the one that slot {slot} ends in at token {length}")
         if r < 0:
             raise ValueError(f"fork(slot={slot}, length={length}) is invalid ({r})")
-        for pool in self.state_pools.values():
-            pool[:, r].copy_(pool[:, slot])
+        if length > 0:                        # (without tokens it is zero, whatever the slot's last request left)
+            for pool in self.state_pools.values():
+                pool[:, r].copy_(pool[:, slot])
+            self._state_came[r] = self.generation(r)
         return r
+
+    def has_state(self, slot: int) -> bool:
+        """Whether the request in the slot was forked, its fixed-size state with it: its first step does not start from zero."""
+        return self._state_came.get(slot) == self.generation(slot)
 
     def compact(self) -> int:
         """Moves the pages in use to the lowest numbers of every group's pool, contents and tables; returns how many moved.

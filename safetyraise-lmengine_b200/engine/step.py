@@ -161,11 +161,9 @@ class Engine:
         fill are shared, the one they end in and the fixed-size state are copied (CacheManager.fork).  Returns its slot."""
         with torch.cuda.device(self.mctx.device):
             if self.cache.state_pools and slot < len(self._slot_generation) \
-                    and self._slot_generation[slot] != self.cache.generation(slot):
+                    and self._slot_generation[slot] != self.cache.generation(slot) and not self.cache.has_state(slot):
                 raise ShapeError(f"slot {slot} has run no step yet: its fixed-size state is another request's")
-            made = self.cache.fork(slot, length)
-        self._slot_generation[made] = self.cache.generation(made)      # its state is set: not to be zeroed at its first step
-        return made
+            return self.cache.fork(slot, length)
 
     # ---- the step -------------------------------------------------------------
     def _validate(self, entries: Sequence[StepEntry]):
@@ -397,10 +395,13 @@ class Engine:
 
     def _greet_new_occupants(self, entries, generations) -> None:
         """A slot that changed hands since this engine last ran it starts from a zero fixed-size state,
-        whoever opened it (this engine, or the scheduler when it admits or re-admits a request)."""
+        whoever opened it (this engine, or the scheduler when it admits or re-admits a request), unless it was
+        forked: then its state came with it."""
         for e, g in zip(entries, generations):
             if g != self._slot_generation[e.slot]:
                 self._slot_generation[e.slot] = g
+                if self.cache.has_state(e.slot):
+                    continue
                 for pool in self.cache.state_pools.values():
                     pool[:, e.slot].zero_()
 
