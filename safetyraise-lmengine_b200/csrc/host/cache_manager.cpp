@@ -1,6 +1,7 @@
 #include "cache_manager.hpp"
 
 #include <algorithm>
+#include <utility>
 
 namespace srlm {
 
@@ -166,11 +167,13 @@ int CacheManager::fork(int slot, int len, std::vector<PageCopy>* copies) {
       if (t[p] < 0) return -3;
     if (len % grp.spec.page_size && grp.free_list.empty()) return -5;
   }
-  const int made = open_request();
-  if (made < 0) return -4;
-  const Slot& from = slots_[slot];
-  Slot& to = slots_[made];
+  if (free_slots_.empty()) return -4;
+  // the memory it takes first: behind the opening nothing can fail
+  copies->reserve(copies->size() + groups_.size());
+  Slot& to = slots_[free_slots_.back()];
   for (size_t g = 0; g < groups_.size(); ++g) to.tables[g].reserve(ceil_div(len, groups_[g].spec.page_size));
+  const int made = open_request();
+  const Slot& from = slots_[slot];
   for (size_t g = 0; g < groups_.size(); ++g) {
     Group& grp = groups_[g];
     const int full = len / grp.spec.page_size;
@@ -199,6 +202,7 @@ int CacheManager::unshare(int slot, int len, std::vector<PageCopy>* copies) {
   };
   for (size_t g = 0; g < groups_.size(); ++g)
     if (shared(g) && groups_[g].free_list.empty()) return 0;
+  copies->reserve(copies->size() + groups_.size());
   for (size_t g = 0; g < groups_.size(); ++g) {
     if (!shared(g)) continue;
     int32_t& mine = s.tables[g][len / groups_[g].spec.page_size];
@@ -211,28 +215,38 @@ int CacheManager::unshare(int slot, int len, std::vector<PageCopy>* copies) {
 }
 
 int CacheManager::compact(std::vector<PageCopy>* copies) {
+  // every group's moves first, with what memory they take: behind them nothing can fail
+  std::vector<std::vector<int32_t>> now(groups_.size());       // the number that each page will have
   int moved = 0;
+  for (size_t g = 0; g < groups_.size(); ++g) {
+    const Group& grp = groups_[g];
+    int used = 0;
+    for (int32_t h : grp.holders) used += h > 0;
+    now[g].resize(grp.spec.num_pages);
+    int32_t hole = 0;
+    for (int32_t p = 0; p < grp.spec.num_pages; ++p) {
+      now[g][p] = p;
+      if (p < used || grp.holders[p] == 0) continue;
+      while (grp.holders[hole] > 0) ++hole;            // below `used`: as many holes there as pages in use beyond
+      copies->push_back(PageCopy{static_cast<int32_t>(g), p, hole});
+      now[g][p] = hole++;
+      ++moved;
+    }
+  }
   for (size_t g = 0; g < groups_.size(); ++g) {
     Group& grp = groups_[g];
     int used = 0;
     for (int32_t h : grp.holders) used += h > 0;
-    std::vector<int32_t> now(grp.spec.num_pages);
-    int32_t hole = 0;
-    for (int32_t p = 0; p < grp.spec.num_pages; ++p) {
-      now[p] = p;
-      if (p < used || grp.holders[p] == 0) continue;
-      while (grp.holders[hole] > 0) ++hole;            // below `used`: as many holes there as pages in use beyond
-      now[p] = hole;
-      grp.holders[hole] = grp.holders[p];
-      grp.holders[p] = 0;
-      grp.ever_used[hole] = 1;
-      copies->push_back(PageCopy{static_cast<int32_t>(g), p, hole});
-      ++moved;
+    for (int32_t p = used; p < grp.spec.num_pages; ++p) {
+      const int32_t to = now[g][p];
+      if (to == p) continue;
+      std::swap(grp.holders[to], grp.holders[p]);
+      grp.ever_used[to] = 1;
     }
     for (Slot& s : slots_)
       for (int32_t& p : s.tables[g])
-        if (p >= 0) p = now[p];
-    grp.free_list.clear();
+        if (p >= 0) p = now[g][p];
+    grp.free_list.clear();                             // (its memory stays)
     for (int32_t p = grp.spec.num_pages - 1; p >= used; --p) grp.free_list.push_back(p);
   }
   return moved;
