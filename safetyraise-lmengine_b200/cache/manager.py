@@ -97,6 +97,7 @@ def runtime():
         for name, numbers in (("fork", 2), ("unshare", 2), ("compact", 0)):
             fn = getattr(lib, "srlm_cache_" + name)
             fn.restype, fn.argtypes = C.c_int, [C.c_void_p] + [C.c_int] * numbers + [at, C.c_int, C.POINTER(C.c_int)]
+        lib.srlm_cache_plan.argtypes = [C.c_void_p] + [C.c_int] * 3 + [at, C.c_int, C.POINTER(C.c_int)]
         lib.srlm_cache_destroy.argtypes = [C.c_void_p]
         lib.srlm_cache_reuse_counts.argtypes = [C.c_void_p, C.POINTER(C.c_int64), C.POINTER(C.c_int64)]
         lib.srlm_sched_destroy.argtypes = [C.c_void_p]
@@ -212,22 +213,31 @@ class CacheManager:
             raise ValueError(f"truncate(slot={slot}, len={length}) is invalid ({r})")
 
     # ---- pages in several requests' tables ----------------------------------------
+    _PAGE_CALLS = {"fork": 0, "unshare": 1, "compact": 2}
+
     def _with_copies(self, what: str, room: int, *args) -> int:
-        """Runs a native call that names pages to copy and copies them, in every pool of their groups, on the current stream."""
-        copies, n = np.empty((max(room, 1), 3), dtype=np.int32), C.c_int()
-        r = getattr(self._lib, "srlm_cache_" + what)(self._h, *args, copies.ctypes.data, max(room, 1), C.byref(n))
+        """Runs a native call that names pages to copy, and copies them, in every pool of their groups, on the current stream.
+        The copies come first, into pages that are nobody's yet: one that cannot be made leaves the tables as they are."""
+        room = max(room, 1)
+        copies, n = np.empty((room, 3), dtype=np.int32), C.c_int()
+        slot, length = args or (0, 0)
+        r = self._lib.srlm_cache_plan(self._h, self._PAGE_CALLS[what], slot, length, copies.ctypes.data, room, C.byref(n))
         if r < 0:
             return r
-        copies = copies[:n.value]
-        if self.device is not None and len(copies):
-            from ..kernels import ops
-            with torch.cuda.device(self.device):
-                for g, spec in enumerate(self._paged):
-                    mine = copies[copies[:, 0] == g]
-                    for pools in (self.kv_pools, self.k_pools, self.v_pools):
-                        if len(mine) and spec.name in pools:
-                            ops.copy_pages(pools[spec.name], mine[:, 1], mine[:, 2])
-        return r
+        self._copy(copies[:n.value])
+        return getattr(self._lib, "srlm_cache_" + what)(self._h, *args, copies.ctypes.data, room, C.byref(n))
+
+    def _copy(self, copies: np.ndarray) -> None:
+        """Rows of (group, source page, destination page)."""
+        if self.device is None or not len(copies):
+            return
+        from ..kernels import ops
+        with torch.cuda.device(self.device):
+            for g, spec in enumerate(self._paged):
+                mine = copies[copies[:, 0] == g]
+                for pools in (self.kv_pools, self.k_pools, self.v_pools):
+                    if len(mine) and spec.name in pools:
+                        ops.copy_pages(pools[spec.name], mine[:, 1], mine[:, 2])
 
     def fork(self, slot: int, length: Optional[int] = None) -> int:
         """A new request that begins with the first ``length`` tokens (default: all committed ones) of the one in ``slot``;
@@ -247,8 +257,12 @@ class CacheManager:
         if r < 0:
             raise ValueError(f"fork(slot={slot}, length={length}) is invalid ({r})")
         if length > 0:                        # (without tokens it is zero, whatever the slot's last request left)
-            for pool in self.state_pools.values():
-                pool[:, r].copy_(pool[:, slot])
+            try:
+                for pool in self.state_pools.values():
+                    pool[:, r].copy_(pool[:, slot])
+            except Exception:
+                self.close_request(r)
+                raise
             self._state_came[r] = self.generation(r)
         return r
 

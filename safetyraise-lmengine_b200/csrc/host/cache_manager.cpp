@@ -156,7 +156,7 @@ int CacheManager::truncate(int slot, int len) {
   return 0;
 }
 
-int CacheManager::fork(int slot, int len, std::vector<PageCopy>* copies) {
+int CacheManager::fork(int slot, int len, std::vector<PageCopy>* copies, bool plan) {
   if (!valid(slot) || len < 0) return -1;
   if (len > slots_[slot].length) return -2;
   for (size_t g = 0; g < groups_.size(); ++g) {
@@ -170,6 +170,13 @@ int CacheManager::fork(int slot, int len, std::vector<PageCopy>* copies) {
   if (free_slots_.empty()) return -4;
   // the memory it takes first: behind the opening nothing can fail
   copies->reserve(copies->size() + groups_.size());
+  if (plan) {
+    for (size_t g = 0; g < groups_.size(); ++g)
+      if (len % groups_[g].spec.page_size)
+        copies->push_back(PageCopy{static_cast<int32_t>(g), slots_[slot].tables[g][len / groups_[g].spec.page_size],
+                                   groups_[g].free_list.back()});
+    return free_slots_.back();
+  }
   Slot& to = slots_[free_slots_.back()];
   for (size_t g = 0; g < groups_.size(); ++g) to.tables[g].reserve(ceil_div(len, groups_[g].spec.page_size));
   const int made = open_request();
@@ -192,7 +199,7 @@ int CacheManager::fork(int slot, int len, std::vector<PageCopy>* copies) {
   return made;
 }
 
-int CacheManager::unshare(int slot, int len, std::vector<PageCopy>* copies) {
+int CacheManager::unshare(int slot, int len, std::vector<PageCopy>* copies, bool plan) {
   if (!valid(slot) || len < 0 || len > slots_[slot].reserved) return -1;
   Slot& s = slots_[slot];
   auto shared = [&](size_t g) {
@@ -206,15 +213,16 @@ int CacheManager::unshare(int slot, int len, std::vector<PageCopy>* copies) {
   for (size_t g = 0; g < groups_.size(); ++g) {
     if (!shared(g)) continue;
     int32_t& mine = s.tables[g][len / groups_[g].spec.page_size];
+    copies->push_back(PageCopy{static_cast<int32_t>(g), mine, groups_[g].free_list.back()});
+    if (plan) continue;
     const int32_t page = take(groups_[g]);
-    copies->push_back(PageCopy{static_cast<int32_t>(g), mine, page});
     give(groups_[g], mine);
     mine = page;
   }
   return 1;
 }
 
-int CacheManager::compact(std::vector<PageCopy>* copies) {
+int CacheManager::compact(std::vector<PageCopy>* copies, bool plan) {
   // every group's moves first, with what memory they take: behind them nothing can fail
   std::vector<std::vector<int32_t>> now(groups_.size());       // the number that each page will have
   int moved = 0;
@@ -233,6 +241,7 @@ int CacheManager::compact(std::vector<PageCopy>* copies) {
       ++moved;
     }
   }
+  if (plan) return moved;
   for (size_t g = 0; g < groups_.size(); ++g) {
     Group& grp = groups_[g];
     int used = 0;

@@ -56,16 +56,18 @@ class CacheManager {
   // what its window still covers: returns <0 then).  -4: len ends inside a page that another
   // request holds too; unshare() first.
   int truncate(int slot, int len);
+  // The three calls below name pages whose contents somebody has to copy.  With plan they only do that, and return what they would:
+  // the copies can be made first, into pages that are nobody's yet, and the call itself, which names the same ones, once they are.
   // A new request that begins with the first len tokens of slot's: its slot, with the pages that len fills shared
   // and a copy of the one that it ends in (added to *copies).  -1 slot not open, -2 len is beyond its length, -3 a window
   // has passed pages that len needs, -4 no slot free, -5 no page free (nothing changed in either case).
-  int fork(int slot, int len, std::vector<PageCopy>* copies);
+  int fork(int slot, int len, std::vector<PageCopy>* copies, bool plan = false);
   // Makes the page that len ends in the slot's own in every group, by a copy (added to *copies) where another request
   // holds it too: 1 done, 0 not enough free pages (nothing changed), <0 bad arguments.
-  int unshare(int slot, int len, std::vector<PageCopy>* copies);
+  int unshare(int slot, int len, std::vector<PageCopy>* copies, bool plan = false);
   // Puts the pages in use together at the lowest numbers, in every group: tables as after the copies that are added to
   // *copies (none reads a page that another writes).  The number of pages moved.
-  int compact(std::vector<PageCopy>* copies);
+  int compact(std::vector<PageCopy>* copies, bool plan = false);
 
   int length(int slot) const;
   int reserved_tokens(int slot) const;

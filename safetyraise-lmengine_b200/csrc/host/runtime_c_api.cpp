@@ -29,19 +29,21 @@ int srlm_cache_fit_tokens(void* c, int slot, int n) { return static_cast<CacheMa
 int srlm_cache_commit(void* c, int slot, int n) { return static_cast<CacheManager*>(c)->commit(slot, n); }
 int srlm_cache_truncate(void* c, int slot, int n) { return static_cast<CacheManager*>(c)->truncate(slot, n); }
 // At most `room` copies are there: fork and unshare make one a group at most, compact one a page.
-static int with_copies(CacheManager* m, int32_t* out, int room, int* n, bool pages, int (*what)(CacheManager*, int, int, std::vector<srlm::PageCopy>*),
-                       int slot, int len) {
+enum PageCall { FORK = 0, UNSHARE = 1, COMPACT = 2 };
+static int with_copies(void* c, int call, bool plan, int slot, int len, int32_t* out, int room, int* n) {
+  CacheManager* m = static_cast<CacheManager*>(c);
   *n = 0;
   int64_t most = 0;
-  for (int g = 0; g < m->num_groups(); ++g) most += pages ? m->num_pages(g) : 1;
+  for (int g = 0; g < m->num_groups(); ++g) most += call == COMPACT ? m->num_pages(g) : 1;
   if (most > room) return -9;
   try {
     std::vector<srlm::PageCopy> copies;
     copies.reserve(most);
-    const int r = what(m, slot, len, &copies);
-    for (const srlm::PageCopy& c : copies) {
+    const int r = call == FORK ? m->fork(slot, len, &copies, plan) : call == UNSHARE ? m->unshare(slot, len, &copies, plan)
+                                                                                    : m->compact(&copies, plan);
+    for (const srlm::PageCopy& p : copies) {
       int32_t* row = out + 3 * (*n)++;
-      row[0] = c.group; row[1] = c.src; row[2] = c.dst;
+      row[0] = p.group; row[1] = p.src; row[2] = p.dst;
     }
     return r;
   } catch (...) {
@@ -49,16 +51,14 @@ static int with_copies(CacheManager* m, int32_t* out, int room, int* n, bool pag
   }
 }
 int srlm_cache_fork(void* c, int slot, int len, int32_t* copies, int room, int* n) {
-  return with_copies(static_cast<CacheManager*>(c), copies, room, n, false,
-                     [](CacheManager* m, int s, int l, std::vector<srlm::PageCopy>* v) { return m->fork(s, l, v); }, slot, len);
+  return with_copies(c, FORK, false, slot, len, copies, room, n);
 }
 int srlm_cache_unshare(void* c, int slot, int len, int32_t* copies, int room, int* n) {
-  return with_copies(static_cast<CacheManager*>(c), copies, room, n, false,
-                     [](CacheManager* m, int s, int l, std::vector<srlm::PageCopy>* v) { return m->unshare(s, l, v); }, slot, len);
+  return with_copies(c, UNSHARE, false, slot, len, copies, room, n);
 }
-int srlm_cache_compact(void* c, int32_t* copies, int room, int* n) {
-  return with_copies(static_cast<CacheManager*>(c), copies, room, n, true,
-                     [](CacheManager* m, int, int, std::vector<srlm::PageCopy>* v) { return m->compact(v); }, 0, 0);
+int srlm_cache_compact(void* c, int32_t* copies, int room, int* n) { return with_copies(c, COMPACT, false, 0, 0, copies, room, n); }
+int srlm_cache_plan(void* c, int call, int slot, int len, int32_t* copies, int room, int* n) {
+  return call < FORK || call > COMPACT ? -1 : with_copies(c, call, true, slot, len, copies, room, n);
 }
 int srlm_cache_length(void* c, int slot) { return static_cast<CacheManager*>(c)->length(slot); }
 int srlm_cache_reserved(void* c, int slot) { return static_cast<CacheManager*>(c)->reserved_tokens(slot); }

@@ -23,6 +23,8 @@ int srlm_cache_truncate(void* cache, int slot, int len);
 int srlm_cache_fork(void* cache, int slot, int len, int32_t* copies, int room, int* n);
 int srlm_cache_unshare(void* cache, int slot, int len, int32_t* copies, int room, int* n);
 int srlm_cache_compact(void* cache, int32_t* copies, int room, int* n);
+/* What fork (call 0), unshare (1) or compact (2; slot and len count for nothing) would return and copy now; nothing changes. */
+int srlm_cache_plan(void* cache, int call, int slot, int len, int32_t* copies, int room, int* n);
 int srlm_cache_length(void* cache, int slot);
 int srlm_cache_reserved(void* cache, int slot);
 int srlm_cache_generation(void* cache, int slot);
