@@ -3,7 +3,7 @@
 //
 // An entry e has q_len tokens (cu_q) and kv_len keys in its pages, the last q_len of them the tokens' own; start = kv_len -
 // q_len keys are committed.  The row of token i and head h sees
-//     a committed key j < start       iff there is no window, or j > positions[token] - window
+//     a committed key j < start       iff there is no window, or j > positions[token] - window, start <= positions[token] < kv_len
 //     the key start + k of token k    iff bit k % 32 of mask[token][k / 32] is set
 // and nothing else; o = sum_j softmax_j(scale q . k_j) v_j over what it sees, zeros where it sees nothing.
 //
@@ -39,7 +39,7 @@
 namespace srlm {
 namespace tree {
 
-enum ErrorCode : int { ERR_PAGE = 71, ERR_ENTRY = 72 };
+enum ErrorCode : int { ERR_PAGE = 71, ERR_ENTRY = 72, ERR_POSITION = 75 };
 
 struct Args {
   const void* q;
@@ -296,9 +296,14 @@ struct Sight {
   }
 };
 
-// The first committed key that a token's window leaves it (a position in front of the token's own place counts as that place).
-__device__ __forceinline__ int first_key_of(const Args& a, int token, int start) {
-  return a.window > 0 ? max(0, max(a.positions[token], start) - a.window + 1) : 0;
+// The first committed key that a token's window leaves it.  A position outside [start, kv_len) is none of the entry's: it raises the
+// error word and counts as the nearest of them.  (Which tiles every row sees whole, and which the entry needs at all, is decided by those
+// two bounds; the entry's last tile is never one of the former, so each row comes by here.)
+__device__ __forceinline__ int first_key_of(const Args& a, int token, int start, int kv_len) {
+  if (a.window <= 0) return 0;
+  const int given = a.positions[token], position = min(max(given, start), kv_len - 1);
+  if (position != given) atomicExch(a.err_flag, ERR_POSITION);
+  return max(0, position - a.window + 1);
 }
 
 // The flat row of key j of KV head kvh in the pools [pages, kv heads, page size, head size]; a page that is not in the pool
@@ -347,7 +352,7 @@ template <typename T, int KEYS>
 __device__ __noinline__ float loose_values(const Args& a, int start, int kv_len, const int* table, int kvh, int token, int d, int tile_lo,
                                            int tile_hi) {
   float sum = 0.f;
-  const int lo = first_key_of(a, token, start);
+  const int lo = first_key_of(a, token, start, kv_len);
   const T* v = (const T*)a.v_cache;
   for (int j0 = tile_lo * KEYS; j0 < tile_hi * KEYS && j0 < kv_len; j0 += 32) {
     if (j0 / KEYS * KEYS + KEYS <= start && (a.window <= 0 || j0 / KEYS * KEYS >= kv_len - a.window)) continue;

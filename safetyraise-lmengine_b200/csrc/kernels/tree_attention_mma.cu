@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(M_THREADS, mma_blocks(HD_MAX)) tree_mma_kernel
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       token[i] = x.q0 + min(r0 + ra + 8 * i, x.q_len * g - 1) / g;
-      lo[i] = first_key_of(a, token[i], x.start);
+      lo[i] = first_key_of(a, token[i], x.start, x.kv_len);
     }
     const bool live = row_warp * 16 < rows;
 

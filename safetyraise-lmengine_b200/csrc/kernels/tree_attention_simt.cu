@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(S_THREADS, simt_blocks(DIMS, KEY_WARPS)) tree_
           for (int o = 0; o < PER; ++o) {
             const int token = x.q0 + (r0 + min(rows0 + o, rows - 1)) / g;
             sight[o].words(a, token, j0, x.start);
-            lo[o] = first_key_of(a, token, x.start);
+            lo[o] = first_key_of(a, token, x.start, x.kv_len);
           }
 #pragma unroll
           for (int o = 0; o < PER; ++o) {

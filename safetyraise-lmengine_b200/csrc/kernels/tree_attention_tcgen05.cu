@@ -335,7 +335,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (!plain && live) {
           Sight<4> sight;
           sight.words(a, token, j0, x.start);
-          sight.bits(bits, j0, x.start, x.kv_len, first_key_of(a, token, x.start));
+          sight.bits(bits, j0, x.start, x.kv_len, first_key_of(a, token, x.start, x.kv_len));
         }
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[i], done & 1, a.err_flag, 87));
         if (!ok) break;

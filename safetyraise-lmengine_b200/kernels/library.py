@@ -910,10 +910,11 @@ class KernelLibrary:
         [n, pages of an entry], cu_q int32 [n + 1], kv_lens int32 [n]; mask int32 [T, words] as ``draft_tree`` makes it
         (any other mask will do: bits of any of the entry's tokens, the token's own among them or not; a token that sees
         nothing has zeros).  max_q_len: no entry has more tokens.  window > 0: a token sees the committed keys less than
-        window in front of its position (positions int32 [T] is wanted then; the mask carries the window among the
-        tokens).  Rows of q behind cu_q[n] are not read and theirs of out are left as they are.  What stands in places
-        of the cache that a token does not see never reaches its row.  A page number outside the pool, or lengths that
-        contradict one another, raise the error word (such an entry's rows are left, such a page is read as page 0)."""
+        window in front of its position (positions int32 [T] is wanted then, from the entry's kv_lens - its tokens to kv_lens - 1,
+        as ``draft_tree`` makes them; the mask carries the window among the tokens).  Rows of q behind cu_q[n] are not read and theirs of out are left as they are.  What stands in places
+        of the cache that a token does not see never reaches its row.  A page number outside the pool, lengths that
+        contradict one another, or a position under a window that is none of the entry's, raise the error word (such a page is
+        read as page 0, such an entry's rows are left, such a position counts as the nearest of the entry's)."""
         what, i32, here, dt = "tree_attention", torch.int32, self._here(), q.dtype
         T, n, pages = q.shape[0], kv_lens.shape[0], k_cache.shape[0]
         code = dtype_code(dt)

@@ -53,3 +53,29 @@ def test_pools_of_one_byte_numbers():
     with pytest.raises(ShapeError, match="odd address"):
         ops.keep_drafts(pool, ints([[2]]), ints([0, 4]), ints([4]), ints([[0, 3]]), ints([2]))
     assert torch.equal(flat, was)
+
+
+@pytest.mark.parametrize("dt, hd, ps", [(torch.bfloat16, 128, 16), (torch.bfloat16, 64, 8), (torch.bfloat16, 80, 16), (torch.float32, 64, 16)])
+@pytest.mark.parametrize("tokens", [3, 40])
+def test_positions_that_are_none_of_the_entry_s(dt, hd, ps, tokens):
+    """Under a window a position in front of the entry's first token, or behind its last key, raises the error word and counts as
+    the nearest that is the entry's, wherever tiles begin and end."""
+    dev = torch.device(DEV)
+    for ctx, window in ((900, 200), (516, 37), (20, 300)):
+        c = Case([tokens, 5], [ctx, 300], 8, 2, hd, ps, dt, window=window, seed=ctx)
+        ops.gemm_error_flag(dev)
+        c.run()
+        c.check()
+        assert ops.gemm_error_flag(dev) == 0
+        right = c.positions.clone()
+        for wrong, nearest in ((ctx + tokens, ctx + tokens - 1), (ctx + tokens + 150, ctx + tokens - 1), (2 ** 31 - 1, ctx + tokens - 1),
+                               (ctx - 1, ctx), (ctx - 70, ctx), (-2 ** 31, ctx)):
+            at = tokens // 2
+            c.positions[at] = nearest
+            want = c.run().clone()
+            assert ops.gemm_error_flag(dev) == 0
+            c.positions[at] = wrong
+            c.run()
+            assert ops.gemm_error_flag(dev) != 0, wrong
+            assert torch.equal(c.out, want), wrong
+            c.positions.copy_(right)
