@@ -294,13 +294,13 @@ __global__ void __launch_bounds__(M_THREADS, mma_blocks(HD_MAX)) tree_mma_kernel
       }
     }
     __syncthreads();                                             // before the next piece's rows and tiles
-    if (loose) {                                                 // (what a row sees of them outweighs all the rest)
+    if (loose) {                                                 // (what a row sees of them, on top of the rest: that may hold some too)
       for (int i = tid; i < rows * hd; i += M_THREADS) {
         const int row = i / hd, d = i - row * hd;
         const float v = loose_values<bf16, M_KEYS>(a, x.start, x.kv_len, table, w.kvh, x.q0 + (r0 + row) / g, d, w.tile_lo, w.tile_hi);
         if (isfinite(v)) continue;
-        if (whole) out_of(row)[d] = from_float<bf16>(v);
-        else a.part_o[(slab * hd + d) * ROWS + row] = v;
+        if (whole) out_of(row)[d] = from_float<bf16>(to_float(out_of(row)[d]) + v);
+        else a.part_o[(slab * hd + d) * ROWS + row] += v;
       }
       __syncthreads();
     }

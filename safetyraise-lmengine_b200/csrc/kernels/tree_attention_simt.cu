@@ -276,15 +276,16 @@ __global__ void __launch_bounds__(S_THREADS, simt_blocks(DIMS, KEY_WARPS)) tree_
       }
     }
     __syncthreads();                                       // before the next piece's places and rows
-    if (loose_sh) {                                        // (what a row sees of them outweighs all the rest)
+    if (loose_sh) {                                        // (what a row sees of them, on top of the rest: that may hold some too)
       const bool whole = w.begins && w.ends;
       const size_t slab = slab_of(blockIdx.x, w.begins);
       for (int i = tid; i < rows * a.hd; i += S_THREADS) {
         const int row = i / a.hd, d = i - row * a.hd, r = r0 + row;
         const float v = loose_values<T, S_KEYS>(a, x.start, x.kv_len, table, w.kvh, x.q0 + r / g, d, w.tile_lo, w.tile_hi);
         if (isfinite(v)) continue;
-        if (whole) ((T*)a.out)[((size_t)(x.q0 + r / g) * a.nq + w.kvh * g + r % g) * a.hd + d] = from_float<T>(v);
-        else a.part_o[(slab * a.hd + d) * ROWS + row] = v;
+        T* dst = (T*)a.out + ((size_t)(x.q0 + r / g) * a.nq + w.kvh * g + r % g) * a.hd + d;
+        if (whole) *dst = from_float<T>(to_float(*dst) + v);
+        else a.part_o[(slab * a.hd + d) * ROWS + row] += v;
       }
       __syncthreads();
     }

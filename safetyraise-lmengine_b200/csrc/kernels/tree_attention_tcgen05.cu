@@ -458,14 +458,14 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             for (int j = 0; j < 32; ++j) a.part_o[(slab * HD + c + j) * T_ROWS + row] = o[j];
           }
         }
-        if (loose_sh && mine)                      // (what a row sees of them outweighs all the rest)
+        if (loose_sh && mine)                      // (what a row sees of them, on top of the rest: that may hold some too)
 #pragma unroll 1
           for (int c = i * (HD / 2); c < (i + 1) * (HD / 2); ++c) {
             const float v = loose_values<bf16, T_KEYS>(a, x.start, x.kv_len, a.block_table + (size_t)w.e * a.table_stride, w.kvh, token,
                                                        c, w.tile_lo, w.tile_hi);
             if (!isfinite(v)) {
-              if (whole) dst[c] = from_float<bf16>(v);
-              else a.part_o[(slab * HD + c) * T_ROWS + row] = v;
+              if (whole) dst[c] = from_float<bf16>(to_float(dst[c]) + v);
+              else a.part_o[(slab * HD + c) * T_ROWS + row] += v;
             }
           }
         fence_before();

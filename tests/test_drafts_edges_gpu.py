@@ -79,3 +79,28 @@ def test_positions_that_are_none_of_the_entry_s(dt, hd, ps, tokens):
             assert ops.gemm_error_flag(dev) != 0, wrong
             assert torch.equal(c.out, want), wrong
             c.positions.copy_(right)
+
+
+@pytest.mark.parametrize("dt, hd, ps", [(torch.bfloat16, 128, 16), (torch.bfloat16, 64, 8), (torch.bfloat16, 80, 16), (torch.float32, 64, 16)])
+@pytest.mark.parametrize("tokens, ctx", [(20, 600), (5, 200), (20, 5000)])
+def test_values_that_are_no_numbers_add_up(dt, hd, ps, tokens, ctx):
+    """Of a committed key that every row sees, and of a drafted one that some see: NaN stays NaN beside an infinity, and infinities of
+    both signs make NaN."""
+    c = Case([tokens], [ctx], 8, 2, hd, ps, dt, seed=3)
+
+    def put(j, d, value):
+        c.v[c.tables[0][j // ps], :, j % ps, d] = value
+
+    node = 3
+    sees = torch.from_numpy(c.seen[0][:, node]).to(DEV)
+    assert sees.any() and not sees.all()
+    early = 10
+    put(early, 3, math.nan), put(early, 7, -math.inf), put(early, 9, math.inf)
+    for d in (3, 5, 7, 9):
+        put(ctx + node, d, math.inf)
+    out = c.run().view(tokens, 8, hd).float()
+    assert out[..., 3].isnan().all()
+    assert (out[sees][..., 5] == math.inf).all() and out[~sees][..., 5].isfinite().all()
+    assert out[sees][..., 7].isnan().all() and (out[~sees][..., 7] == -math.inf).all()
+    assert (out[..., 9] == math.inf).all()
+    assert out[..., 0].isfinite().all()
