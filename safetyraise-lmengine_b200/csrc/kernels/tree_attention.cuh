@@ -485,14 +485,15 @@ inline void launch_merge(const Args& a, int blocks, cudaStream_t stream) {
 }
 
 // Lets a kernel have `bytes` of shared memory, once a device (the attribute stays with the kernel; each kernel has a `have` of its own).
-inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<int> (&have)[64]) {
+// The same number on every call of a kernel, the most that any of its calls takes: threads that come here together write the same.
+inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<bool> (&have)[64]) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  std::atomic<int>* slot = dev < 64 ? &have[dev] : nullptr;
-  if (slot && slot->load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
+  std::atomic<bool>* slot = dev < 64 ? &have[dev] : nullptr;
+  if (slot && slot->load(std::memory_order_relaxed)) return cudaSuccess;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && slot) slot->store(bytes, std::memory_order_relaxed);
+  if (e == cudaSuccess && slot) slot->store(true, std::memory_order_relaxed);
   return e;
 }
 

@@ -318,10 +318,10 @@ Form mma_form(int hd, int max_rows, int sms) { return Form{mma_blocks(hd) * sms,
 template <int HD_MAX, int KEY_WARPS, int STAGES>
 static int run_form(const Args& a, int blocks, cudaStream_t stream) {
   using F = MmaForm<HD_MAX, KEY_WARPS, STAGES>;
-  const int smem = (int)F::smem(a.hd);
-  static std::atomic<int> have[64];
-  const cudaError_t e = allow_smem((const void*)tree_mma_kernel<HD_MAX, KEY_WARPS, STAGES>, smem, have);
-  if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", smem);
+  const int smem = (int)F::smem(a.hd), most = (int)F::smem(HD_MAX);
+  static std::atomic<bool> have[64];
+  const cudaError_t e = allow_smem((const void*)tree_mma_kernel<HD_MAX, KEY_WARPS, STAGES>, most, have);
+  if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", most);
   launch_pdl(tree_mma_kernel<HD_MAX, KEY_WARPS, STAGES>, dim3(blocks), dim3(M_THREADS), smem, stream, a);
   launch_merge<bf16, F::ROWS, M_KEYS>(a, blocks, stream);
   return launched();

@@ -302,10 +302,10 @@ Form simt_form(int hd, int max_rows, int sms) {
 
 template <typename T, int DIMS, bool COPY, int KEY_WARPS>
 static int run_form(const Args& a, int blocks, cudaStream_t stream) {
-  const int smem = (int)SimtForm<KEY_WARPS>::smem(a.hd);
-  static std::atomic<int> have[64];
-  const cudaError_t e = allow_smem((const void*)tree_simt_kernel<T, DIMS, COPY, KEY_WARPS>, smem, have);
-  if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", smem);
+  const int smem = (int)SimtForm<KEY_WARPS>::smem(a.hd), most = (int)SimtForm<KEY_WARPS>::smem(32 * DIMS);
+  static std::atomic<bool> have[64];
+  const cudaError_t e = allow_smem((const void*)tree_simt_kernel<T, DIMS, COPY, KEY_WARPS>, most, have);
+  if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", most);
   launch_pdl(tree_simt_kernel<T, DIMS, COPY, KEY_WARPS>, dim3(blocks), dim3(S_THREADS), smem, stream, a);
   launch_merge<T, SimtForm<KEY_WARPS>::ROWS, S_KEYS>(a, blocks, stream);
   return launched();

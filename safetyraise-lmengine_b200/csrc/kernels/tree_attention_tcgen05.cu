@@ -506,7 +506,7 @@ static int run_form(const Args& a, int sms, cudaStream_t stream) {
   CUtensorMap mk, mv;
   if (rows > 0x7fffffff || !tensor_map(&mk, a.k_cache, rows, HD, box_rows) || !tensor_map(&mv, a.v_cache, rows, HD, box_rows))
     return refuse(ST_BAD_SIZE, "tree_attention: the caches of %lld rows of %d cannot be mapped", rows, HD);
-  static std::atomic<int> have[64];
+  static std::atomic<bool> have[64];
   const cudaError_t e = allow_smem((const void*)tree_tcgen05_kernel<HD>, TmaForm<HD>::SMEM, have);
   if (e != cudaSuccess) return refuse((int)e, "tree_attention: cannot get %d bytes of shared memory", TmaForm<HD>::SMEM);
   launch_pdl(tree_tcgen05_kernel<HD>, dim3(sms), dim3(T_THREADS), TmaForm<HD>::SMEM, stream, mk, mv, a);

@@ -1,6 +1,7 @@
 """Attention for drafted tokens at its edges: blocks of few rows beside numbers that are none, positions that are none of the
 entry's.  Tolerances: those of ``test_drafts_gpu.Case.check``."""
 import math
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -104,3 +105,28 @@ def test_values_that_are_no_numbers_add_up(dt, hd, ps, tokens, ctx):
     assert out[sees][..., 7].isnan().all() and (out[~sees][..., 7] == -math.inf).all()
     assert (out[..., 9] == math.inf).all()
     assert out[..., 0].isfinite().all()
+
+
+@pytest.mark.parametrize("dt, sizes", [(torch.bfloat16, (144, 256, 160, 240)), (torch.float32, (132, 256, 140, 255))])
+@pytest.mark.parametrize("tokens", [4, 8, 40])
+def test_calls_of_several_threads(dt, sizes, tokens):
+    """Heads of unlike sizes that one kernel takes, from several host threads at once, each on a stream of its own: a call's
+    shared memory is not another's to take away."""
+    cases = [Case([tokens, 3], [100, 40], 4, 2, hd, 20, dt, seed=hd) for hd in sizes]
+    ops.gemm_error_flag(torch.device(DEV))
+
+    def serve(c):
+        torch.cuda.set_device(DEV)
+        outs = []
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                outs.append(c.run().clone())
+        torch.cuda.synchronize()
+        return all(torch.equal(o, outs[0]) for o in outs)
+
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(len(cases)) as pool:
+        assert all(pool.map(serve, cases))
+    for c in cases:
+        c.check()
+    assert ops.gemm_error_flag(torch.device(DEV)) == 0
