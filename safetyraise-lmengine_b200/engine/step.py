@@ -469,16 +469,28 @@ class Engine:
     def revoke(self, prep: PreparedStep) -> None:
         """Takes a launched step back: the fixed-size state of its slots as it was, lengths and pages as
         before the step.  (After ``commit`` a window group may already have let go of pages the old
-        length needs; such a request can only be closed, which is what the generation loop does.)"""
+        length needs; such a request can only be closed, which is what the generation loop does.)  A length
+        inside a page that a fork shares by now takes a page for a copy: where none is free, not among those that the
+        other entries return either, those entries are taken back all the same and ResourceExhausted names the rest, which
+        ``CacheManager.truncate`` takes back once there is a page."""
         with torch.cuda.device(self.mctx.device):
             for name, (idx, saved) in (prep.state_snapshot or {}).items():
                 self.cache.state_pools[name].index_copy_(1, idx, saved)
         prep.state_snapshot = None
-        for e, s in zip(prep.entries, prep.starts):
-            try:
-                self.cache.truncate(e.slot, s)
-            except ValueError:
-                pass
+        left = list(zip(prep.entries, prep.starts))
+        while left:
+            short = []
+            for e, s in left:
+                try:
+                    self.cache.truncate(e.slot, s)
+                except ResourceExhausted:
+                    short.append((e, s))
+                except ValueError:
+                    pass
+            if len(short) == len(left):
+                raise ResourceExhausted("no free page for the copies that slots " + ", ".join(str(e.slot) for e, _ in short)
+                                        + " need to be taken back: they stand behind the step still")
+            left = short
 
     def read_faults(self):
         """The fault words, read from the device (waits for it)."""
