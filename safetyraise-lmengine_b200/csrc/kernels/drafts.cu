@@ -299,6 +299,9 @@ extern "C" int srlm_keep_drafts(void* pool, long long slabs, long long num_pages
   });
 }
 
+// Kernels that a copy of n pages launches.
+extern "C" int srlm_copy_pages_launches(int n) { return n <= 0 ? 0 : n <= COPY_FEW ? 1 : (n + COPY_MANY - 1) / COPY_MANY; }
+
 // pool [slabs, num_pages, page_bytes]; src, dst: host arrays of n page numbers.  No page is written twice, none is both read
 // and written.
 extern "C" int srlm_copy_pages(void* pool, long long slabs, long long num_pages, long long page_bytes, const long long* src,

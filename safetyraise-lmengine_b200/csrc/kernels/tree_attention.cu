@@ -31,10 +31,12 @@ extern "C" long long srlm_tree_attention_workspace(int dtype, int nq, int nkv, i
 
 // q, out [T, nq, hd]; caches [num_pages, nkv, page_size, hd]; block_table [n, table_stride]; cu_q [n + 1]; kv_lens [n]; mask
 // [T, words]; positions [T], or null without a window.  max_q_len: no entry has more tokens.  work: as above says.
+// launches (a host address, or null): how many kernels the call launched.
 extern "C" int srlm_tree_attention(const void* q, const void* k_cache, const void* v_cache, void* out, int dtype, long long num_pages,
                                    const int* block_table, int table_stride, const int* cu_q, const int* kv_lens, const int* mask,
                                    int words, const int* positions, int n, int T, int nq, int nkv, int hd, int page_size, float scale,
-                                   int window, int max_q_len, float* work, int sms, int* err_flag, cudaStream_t stream) {
+                                   int window, int max_q_len, float* work, int sms, int* err_flag, int* launches, cudaStream_t stream) {
+  if (launches) *launches = 0;
   if (n <= 0 || T <= 0) return ST_OK;
   if (srlm_tree_attention_workspace(dtype, nq, nkv, hd, page_size, max_q_len, sms) < 0) return ST_BAD_SIZE;
   if (words <= 0 || table_stride <= 0 || num_pages <= 0 || num_pages > 0x7fffffff || window < 0 || (window > 0 && !positions) || !(scale > 0.f) || !work ||
@@ -61,6 +63,7 @@ extern "C" int srlm_tree_attention(const void* q, const void* k_cache, const voi
   // 16.6 | 14.7 | 15.8; warp level 11.1 | 12.3 | 15.4 and 18.0 | 15.0 | 15.1; float32 13.3 | 15.0 | 18.7 and 22.5 | 20.4 | 22.0).
   const long long keys = (long long)table_stride * page_size, most = (keys + f.keys - 1) / f.keys;
   a.least_tiles = most <= (kind == TCGEN05 ? 6 : kind == MMA ? 4 : 2) ? (int)most : 2;
+  if (launches) *launches = tree::merges(a, f.blocks, f.rows, f.keys) ? 2 : 1;
   if (kind == SIMT) return tree::run_simt(a, dtype, max_rows, sms, stream);
   if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) % 16)
     return refuse(ST_BAD_ALIGN, "tree_attention: bfloat16 tensors start on 16-byte boundaries");

@@ -472,12 +472,16 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) tree_merge_kernel(const __gr
   for (int i = 0; i < MERGE_DIMS; ++i)
     if (i < dims) dst[i] = from_float<T>(acc[i]);
 }
-// Not launched where no unit can have several slabs: every unit has at most least_tiles tiles by the block table's width, and there
+// Whether some unit can have several slabs.  None can where every unit has at most least_tiles tiles by the block table's width, and there
 // are no more units than blocks (their parts are whole units then).
+inline bool merges(const Args& a, int blocks, int rows, int keys) {
+  const long long tiles = ((long long)a.table_stride * a.page_size + keys - 1) / keys;
+  const long long units = (long long)a.n * a.nkv * ((a.max_q_len * a.g + rows - 1) / rows);
+  return a.n > 32 || units > blocks || tiles > a.least_tiles;
+}
 template <typename T, int ROWS, int KEYS>
 inline void launch_merge(const Args& a, int blocks, cudaStream_t stream) {
-  const long long keys = (long long)a.table_stride * a.page_size, units = (long long)a.n * a.nkv * ((a.max_q_len * a.g + ROWS - 1) / ROWS);
-  if (a.n <= 32 && units <= blocks && (keys + KEYS - 1) / KEYS <= a.least_tiles) return;
+  if (!merges(a, blocks, ROWS, KEYS)) return;
   constexpr int RL = ROWS < 32 ? ROWS : 32, SPAN = 32 / RL * MERGE_DIMS;
   const int dim_warps = (a.hd + SPAN - 1) / SPAN, turns = std::min(MERGE_TURNS, MERGE_WARPS / dim_warps);
   const int max_rows = std::min(a.max_q_len * a.g, ROWS);

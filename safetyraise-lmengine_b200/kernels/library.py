@@ -840,10 +840,11 @@ class KernelLibrary:
     _INT, _LONG, _AT, _FLOAT = C.c_int, C.c_longlong, C.c_void_p, C.c_float
     _DRAFT_ENTRIES = {
         "srlm_draft_tree": [_AT] * 5 + [_INT] * 4 + [_AT] * 2,
-        "srlm_tree_attention": [_AT] * 4 + [_INT, _LONG, _AT, _INT] + [_AT] * 3 + [_INT, _AT] + [_INT] * 6 + [_FLOAT, _INT, _INT, _AT, _INT, _AT, _AT],
+        "srlm_tree_attention": [_AT] * 4 + [_INT, _LONG, _AT, _INT] + [_AT] * 3 + [_INT, _AT] + [_INT] * 6 + [_FLOAT, _INT, _INT, _AT, _INT, _AT, _AT, _AT],
         "srlm_tree_attention_workspace": [_INT] * 7,
         "srlm_accept_drafts": [_AT] * 4 + [_INT] * 2 + [_AT, _INT] + [_AT] * 4,
         "srlm_keep_drafts": [_AT, _LONG, _LONG, _INT, _INT, _LONG, _AT, _INT] + [_AT] * 3 + [_INT, _AT, _INT, _AT, _AT],
+        "srlm_copy_pages_launches": [_INT],
         "srlm_copy_pages": [_AT, _LONG, _LONG, _LONG, _AT, _AT, _INT, _INT, _AT],
     }
 
@@ -897,6 +898,8 @@ class KernelLibrary:
                 self._at(what, "mask", mask, (positions.shape[0], words), i32, here))
         if positions.shape[0] != T:
             raise ShapeError(f"draft_tree: {T} parents, {positions.shape[0]} positions")
+        if T == 0 or n == 0:
+            return
         self._check(self._entry("srlm_draft_tree")(*args, words, n, T, window, self._gemm_state(parents.device)[1].data_ptr(),
                                                    self._raw_stream(here)), what)
 
@@ -942,9 +945,11 @@ class KernelLibrary:
             self._tree_work[sizes] = need
         # of this call alone: calls on several streams, and graphs recorded apart, share nothing
         work = q.new_empty(need, dtype=torch.float32)
+        launched = C.c_int()
         self._check(self._entry("srlm_tree_attention")(
             *args, code, pages, *ints, n, T, nq, nkv, hd, page_size, scale, window, max_q_len, work.data_ptr(), sms,
-            self._gemm_state(q.device)[1].data_ptr(), self._raw_stream(here)), what)
+            self._gemm_state(q.device)[1].data_ptr(), C.byref(launched), self._raw_stream(here)), what)
+        self.launches += launched.value - 1       # the kernel that adds what several blocks have of a unit
 
     def accept_drafts(self, tokens, parents, targets, cu_q, path, count, next_token):
         """Follows the model's own choice down each entry's tree of drafted tokens.
@@ -963,6 +968,8 @@ class KernelLibrary:
                 self._at(what, "targets", targets, (T,), i32, here), self._at(what, "cu_q", cu_q, (n + 1,), i32, here), n, T,
                 self._at(what, "path", path, (n, room), i32, here), room, self._at(what, "count", count, (n,), i32, here),
                 self._at(what, "next_token", next_token, (n,), i32, here))
+        if n == 0:
+            return
         self._check(self._entry("srlm_accept_drafts")(*args, self._gemm_state(cu_q.device)[1].data_ptr(), self._raw_stream(here)), what)
 
     def _page_pool(self, what, pool, here):
@@ -990,6 +997,8 @@ class KernelLibrary:
         ints = (self._at(what, "block_table", block_table, (n, width), i32, here), width, self._at(what, "cu_q", cu_q, (n + 1,), i32, here),
                 self._at(what, "kv_lens", kv_lens, (n,), i32, here), self._at(what, "path", path, (n, room), i32, here), room,
                 self._at(what, "count", count, (n,), i32, here))
+        if n == 0:
+            return
         self._check(self._entry("srlm_keep_drafts")(at, slabs, pages, nkv, page_size, hd * pool.element_size(), *ints, n,
                                                     self._gemm_state(pool.device)[1].data_ptr(), self._raw_stream(here)), what)
 
@@ -1003,8 +1012,11 @@ class KernelLibrary:
         if n != len(dst):
             raise ShapeError(f"copy_pages: {n} pages to {len(dst)}")
         numbers = [self._page_numbers(x, n, pages) for x in (src, dst)]
+        if n == 0:
+            return
         self._check(self._entry("srlm_copy_pages")(at, slabs, pages, page[0] * page[1] * page[2] * pool.element_size(), numbers[0],
                                                    numbers[1], n, self.sm_count(pool.device), self._raw_stream(here)), what)
+        self.launches += self._entry("srlm_copy_pages_launches")(n) - 1
 
     @staticmethod
     def _page_numbers(x, n, pages):
