@@ -187,7 +187,7 @@ class Engine:
             if e.generation is not None and e.generation != generation:
                 raise ShapeError(f"slot {e.slot} was given to another request since this one opened it "
                                  f"(generation {generation}, the entry holds {e.generation})")
-            if start + n > self.max_context:
+            if start + n > self.max_context and (e.parents is None or start + self._longest_line(e.parents) > self.max_context):
                 raise ShapeError(f"slot {e.slot}: {start}+{n} tokens exceed the context of {self.max_context}")
             if n == 1:                               # a decoded token: no array for one number
                 t = int(e.tokens[0])
@@ -205,6 +205,14 @@ class Engine:
         if total > self.mctx.max_batch_tokens:
             raise ShapeError(f"{total} tokens in one step exceed max_batch_tokens={self.mctx.max_batch_tokens}")
         return slots, lengths, generations
+
+    @staticmethod
+    def _longest_line(parents) -> int:
+        """Tokens on a tree's longest line: what of it counts against the context, for siblings share a position."""
+        lengths: List[int] = []
+        for i, p in enumerate(parents):
+            lengths.append(1 + lengths[p] if 0 <= p < i else 1)
+        return max(lengths, default=0)
 
     def _meta_buffers(self, words: int):
         """A pinned host buffer that no copy in flight still reads, and the device buffer."""
@@ -555,7 +563,8 @@ class Engine:
         one's parent (None: a chain).  Every token sees the request's committed tokens and those it descends from.  The
         walk from the first token goes to the first child whose token is the model's greedy choice behind the one before;
         the tokens on it are committed, their keys and values side by side, and the rest is forgotten.  Each entry
-        gets at least its first token and one token more (``next_token``, not run yet).  A step that fails keeps nothing
+        gets at least its first token and one token more (``next_token``, not run yet).  A tree's longest line must fit the
+        context, all of its tokens the free pages.  A step that fails keeps nothing
         (StepFailed), as in ``step``."""
         self._check_drafts(entries)
         prep = self.prepare([StepEntry(e.slot, e.tokens, range(len(e.tokens)), e.generation, e.parents) for e in entries], drafts=True)

@@ -26,3 +26,26 @@ def test_a_fork_made_by_the_cache_takes_the_fixed_size_state_along(tmp_path_fact
         ref = alone.step([StepEntry(s, new, [len(new) - 1])]).cpu().numpy()[0]
         assert np.abs(row - ref).max() <= TOL["float32"] * np.abs(ref).max()
         alone.close_request(s)
+
+
+def test_a_wide_tree_at_the_end_of_the_context(folder_a):
+    """Its lines fit, its tokens side by side do not; page and table have places for them all, and what is kept is the context's
+    last tokens."""
+    from safetyraise_lmengine_b200 import Engine, StepEntry
+    from safetyraise_lmengine_b200.errors import ShapeError
+    import plain_qwen3
+    cfg, w = plain_qwen3.read_model_folder(folder_a)
+    eng = Engine.from_folder(folder_a, dtype="float32", page_size=4, num_pages=24, max_requests=2, max_batch_tokens=64, max_context=32)
+    prompt = random_tokens(np.random.default_rng(8), 28, cfg["vocab_size"])
+    truth = plain_qwen3.greedy_generate(cfg, w, prompt, 5)
+    s = eng.open_request()
+    assert int(eng.step([StepEntry(s, prompt, [27])]).argmax()) == truth[0]
+    wrong = [(t + 1) % cfg["vocab_size"] for t in truth]
+    # the line of four behind wrong siblings at every place
+    tokens, parents = [truth[0]] + [wrong[1]] * 6 + [truth[1], wrong[2], truth[2], wrong[3], truth[3]], [-1] + [0] * 7 + [7, 7, 9, 9]
+    with pytest.raises(ShapeError):
+        eng.verify([StepEntry(s, tokens + [1], parents=parents + [11])])
+    v, = eng.verify([StepEntry(s, tokens, parents=parents)])
+    assert v.path == [0, 7, 9, 11] and v.next_token == truth[4]
+    assert eng.cache.length(s) == 32 and eng.cache.audit() == 0
+    assert eng.cache.free_pages() == 16
