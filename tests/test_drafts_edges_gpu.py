@@ -130,3 +130,28 @@ def test_calls_of_several_threads(dt, sizes, tokens):
     for c in cases:
         c.check()
     assert ops.gemm_error_flag(torch.device(DEV)) == 0
+
+
+@pytest.mark.parametrize("dt, hd, ps", [(torch.bfloat16, 128, 16), (torch.bfloat16, 64, 8), (torch.bfloat16, 128, 128), (torch.bfloat16, 80, 16),
+                                        (torch.float32, 64, 16)])
+@pytest.mark.parametrize("ctx, window", [(700, 50), (515, 130), (1030, 3)])
+def test_pages_that_a_window_has_passed(dt, hd, ps, ctx, window):
+    """Given back, -1 in the table: not missed, with whatever page 0 holds by now; the first page that the window still needs is."""
+    dev = torch.device(DEV)
+    c = Case([20, 3], [ctx, 40], 8, 2, hd, ps, dt, window=window, seed=ctx)
+    want = c.run().clone()
+    c.check()
+    needed = max(0, ctx - window + 1) // ps
+    assert needed > 0
+    for t in (c.k, c.v):                                           # page 0 is another request's: numbers that would show
+        if 0 not in c.tables[0][needed:].tolist() + c.tables[1].tolist():
+            t[0] = math.nan
+    ops.gemm_error_flag(dev)
+    c.table[0, :needed] = -1
+    c.out.fill_(7.0)
+    c.run()
+    assert ops.gemm_error_flag(dev) == 0
+    assert torch.equal(c.out, want)
+    c.table[0, needed] = -1
+    c.run()
+    assert ops.gemm_error_flag(dev) != 0
