@@ -14,8 +14,12 @@
 // bounds calls of many rows: 1.45 us a tile and stream, of which 0.55 are its exponentials alone, beside 0.9 us of products.  A block
 // stays for all of its pieces: the fetches run ahead across them, and the block count is the SMs'.
 //
-// A weight is rounded to bfloat16 for the product with the values.  O is rescaled only when a row's maximum has grown by more
-// than 2^8: until then the old one stays the reference of the exponentials, and the division by the sum makes it exact.
+// A weight is rounded to bfloat16 for the product with the values, which is what the MMA takes; a row's sum is of the weights before that
+// rounding, each at most 2^-8 of itself from what the product sees.  Outputs are 0.0023 of their size off 64 bits, 0.0017 of it from their
+// own type (the warp-level form, whose sum is of the rounded weights: 0.0021); unpacking the rounded pairs for the sum would be two more
+// instructions a pair in the softmax, which bounds calls of many rows.
+// O is rescaled only when a row's maximum has grown by more than 2^8: until then the old one stays the reference of the exponentials, and
+// the division by the sum makes it exact.
 // Every wait is bounded; one that runs out raises the error word and ends the block's work.
 #include "attention_tcgen05.cuh"
 #include "tree_attention.cuh"
